@@ -18,15 +18,19 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/version.h>
 
+#include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdlib>
 #include <limits>
+#include <utility>
 
 #include "../../include/moonmath_gfx950.h"
 
@@ -56,7 +60,12 @@ struct Abi {
   X(launch_mla_decode_a16w8_paged_dev)                                                                     \
   X(launch_mla_decode_a16w8_multiq_paged_dev)                                                              \
   X(launch_mla_decode_a16w8_paged_blocks_dev)                                                              \
-  X(launch_mla_kv_quantize)
+  X(launch_mla_kv_quantize)                                                                                \
+  X(launch_gqa_kv_write)                                                                                   \
+  X(launch_gqa_kv_read)                                                                                    \
+  X(launch_gqa_decode_paged)                                                                               \
+  X(moonmath_gqa_decode_workspace)                                                                         \
+  X(launch_rope_axes)
 #define MM_FIELD(name) decltype(&::name) name = nullptr;
   MM_ABI(MM_FIELD)
 #undef MM_FIELD
@@ -451,6 +460,278 @@ PyObject* kv_quantize(PyObject*, PyObject* const* x, Py_ssize_t n) {
   });
 }
 
+// A strided GPU tensor whose last dim is contiguous and whose rows lie on 16-byte
+// boundaries, recording no graph.
+const Tensor& rows_tensor(const Tensor& t, at::ScalarType dtype, c10::Device dev, int64_t dim) {
+  plain(t.defined() && t.scalar_type() == dtype && t.layout() == at::kStrided && t.device() == dev && t.dim() == dim &&
+        !at::isTensorSubclassLike(t) && !t.is_neg() && !(t.requires_grad() && c10::GradMode::is_enabled()));
+  plain(t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0);
+  const int64_t es = (int64_t)t.element_size();
+  for (int64_t i = 0; i + 1 < dim; ++i) plain(t.size(i) <= 1 || t.stride(i) * es % 16 == 0);
+  return t;
+}
+
+// No two elements share memory: each dim steps over all that the smaller steps span.
+void one_place_each(const Tensor& t) {
+  std::pair<int64_t, int64_t> d[4];
+  int n = 0;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) d[n++] = {t.stride(i), t.size(i)};
+  std::sort(d, d + n);
+  int64_t span = 1;
+  for (int i = 0; i < n; ++i) {
+    plain(d[i].first >= span);
+    span += d[i].first * (d[i].second - 1);
+  }
+}
+
+bool apart(const Tensor& a, const Tensor& b) {
+  const auto end = [](const Tensor& t) {
+    int64_t last = t.numel() ? 1 : 0;
+    if (t.numel())
+      for (int64_t i = 0; i < t.dim(); ++i) last += t.stride(i) * (t.size(i) - 1);
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) + last * t.element_size();
+  };
+  return end(a) <= reinterpret_cast<uintptr_t>(b.data_ptr()) || end(b) <= reinterpret_cast<uintptr_t>(a.data_ptr());
+}
+
+bool bool_arg(PyObject* o) {
+  plain(PyBool_Check(o));
+  return o == Py_True;
+}
+
+struct GqaCache {
+  Tensor k, v, ks, vs;
+  int blocks, heads, page, D;
+  long long strides[10];
+};
+
+GqaCache gqa_cache(PyObject* k, PyObject* v, PyObject* ks, PyObject* vs, bool written) {
+  GqaCache c{unpack(k), unpack(v), Tensor(), Tensor(), 0, 0, 0, 0, {}};
+  plain(c.k.is_cuda());
+  check_modes();
+  const auto dev = c.k.device();
+  const auto type = c.k.scalar_type();
+  plain(type == at::kBFloat16 || type == at::kFloat8_e4m3fn);
+  const bool fp8 = type == at::kFloat8_e4m3fn;
+  plain((ks != Py_None) == fp8 && (vs != Py_None) == fp8);
+  rows_tensor(c.k, type, dev, 4);
+  rows_tensor(c.v, type, dev, 4);
+  plain(c.v.sizes() == c.k.sizes());
+  c.blocks = as_int(c.k.size(0));
+  c.heads = as_int(c.k.size(1));
+  c.page = as_int(c.k.size(2));
+  c.D = as_int(c.k.size(3));
+  plain(c.blocks >= 1 && c.heads >= 1 && c.page >= 16 && (c.page & (c.page - 1)) == 0 &&
+        (c.D == 64 || c.D == 128 || c.D == 256) && (int64_t)c.blocks * c.page <= (int64_t)1 << 31);
+  if (fp8) {
+    c.ks = unpack(ks);
+    c.vs = unpack(vs);
+    for (const Tensor* t : {&c.ks, &c.vs}) {
+      rows_tensor(*t, at::kFloat, dev, 3);
+      plain(t->sizes() == c.k.sizes().slice(0, 3));
+    }
+  }
+  for (int w = 0; w < 2; ++w) {
+    const Tensor &t = w ? c.v : c.k, &s = w ? c.vs : c.ks;
+    for (int i = 0; i < 3; ++i) c.strides[5 * w + i] = t.stride(i);
+    for (int i = 0; i < 2; ++i) c.strides[5 * w + 3 + i] = fp8 ? s.stride(i) : 0;
+    plain(t.stride(2) <= 1 << 26);
+    if (written) {
+      one_place_each(t);
+      if (fp8) one_place_each(s);
+    }
+  }
+  return c;
+}
+
+// k, v rows of the tokens in `slots`, apart from the cache.
+int64_t gqa_rows(const Tensor& k, const Tensor& v, const Tensor& slots, const GqaCache& c, bool written,
+                 long long* strides) {
+  const auto dev = c.k.device();
+  check_tensor(slots, at::kInt, dev);
+  plain(slots.dim() == 1);
+  int at = 0;
+  for (const Tensor* t : {&k, &v}) {
+    rows_tensor(*t, at::kBFloat16, dev, 3);
+    plain(t->size(0) == slots.size(0) && t->size(1) == c.heads && t->size(2) == c.D);
+    plain(apart(*t, c.k) && apart(*t, c.v));
+    if (written) one_place_each(*t);
+    strides[at++] = t->stride(0);
+    strides[at++] = t->stride(1);
+  }
+  std::copy(c.strides, c.strides + 10, strides + 4);
+  return slots.size(0);
+}
+
+// k, v, k_cache, v_cache, slots, k_scale or None, v_scale or None
+PyObject* gqa_write(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    plain(n == 7);
+    const Tensor &k = unpack(x[0]), &v = unpack(x[1]), &slots = unpack(x[4]);
+    const GqaCache c = gqa_cache(x[2], x[3], x[5], x[6], true);
+    long long st[14];
+    const int64_t N = gqa_rows(k, v, slots, c, false, st);
+    {
+      pybind11::gil_scoped_release no_gil;
+      const c10::DeviceGuard guard(k.device());
+      check_rc(abi.launch_gqa_kv_write(k.data_ptr(), v.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), ptr_or_null(c.ks),
+                                       ptr_or_null(c.vs), slots.data_ptr(), N, c.heads, c.D, c.blocks, c.page, st,
+                                       stream_of(k)),
+               "launch_gqa_kv_write");
+    }
+    Py_RETURN_TRUE;
+  });
+}
+
+// k_cache, v_cache, slots, k_scale or None, v_scale or None, k or None, v or None
+PyObject* gqa_read(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    plain(n == 7);
+    const Tensor& slots = unpack(x[2]);
+    const GqaCache c = gqa_cache(x[0], x[1], x[3], x[4], false);
+    plain(slots.dim() == 1 && slots.device() == c.k.device());
+    Tensor out[2];
+    for (int i = 0; i < 2; ++i)
+      out[i] = x[5 + i] != Py_None
+                   ? unpack(x[5 + i])
+                   : at::empty({slots.size(0), c.heads, c.D}, c.k.options().dtype(at::kBFloat16).requires_grad(false));
+    long long st[14];
+    const int64_t N = gqa_rows(out[0], out[1], slots, c, true, st);
+    {
+      pybind11::gil_scoped_release no_gil;
+      const c10::DeviceGuard guard(c.k.device());
+      check_rc(abi.launch_gqa_kv_read(c.k.data_ptr(), c.v.data_ptr(), ptr_or_null(c.ks), ptr_or_null(c.vs),
+                                      slots.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), N, c.heads, c.D,
+                                      c.blocks, c.page, st, stream_of(c.k)),
+               "launch_gqa_kv_read");
+    }
+    PyObject* pair = PyTuple_New(2);
+    if (!pair) return nullptr;
+    for (int i = 0; i < 2; ++i) {
+      if (x[5 + i] != Py_None) Py_INCREF(x[5 + i]);
+      PyTuple_SET_ITEM(pair, i, x[5 + i] != Py_None ? x[5 + i] : THPVariable_Wrap(out[i]));
+    }
+    return pair;
+  });
+}
+
+// q, k_cache, v_cache, seq_lens, block_table, scale or None, k_scale, v_scale, out or None, return_lse
+PyObject* gqa_decode(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    plain(n == 10);
+    const Tensor &q = unpack(x[0]), &lens = unpack(x[3]), &table = unpack(x[4]);
+    const GqaCache c = gqa_cache(x[1], x[2], x[6], x[7], false);
+    const bool want_lse = bool_arg(x[9]);
+    const auto dev = c.k.device();
+    const int64_t dims = q.dim();
+    plain(dims == 3 || dims == 4);
+    rows_tensor(q, at::kBFloat16, dev, dims);
+    plain(q.size(-1) == c.D);
+    const int B = as_int(q.size(0)), q_len = dims == 4 ? as_int(q.size(1)) : 1, Hq = as_int(q.size(dims - 2));
+    plain(q_len >= 1 && q_len <= 8 && Hq >= 1 && Hq % c.heads == 0);
+    check_tensor(lens, at::kInt, dev);
+    plain(lens.dim() == 1 && lens.size(0) == B);
+    plain(table.scalar_type() == at::kInt && table.layout() == at::kStrided && table.device() == dev &&
+          !at::isTensorSubclassLike(table) && !table.is_neg() && table.dim() == 2 && table.size(0) == B &&
+          table.size(1) >= 1 && (table.size(1) == 1 || table.stride(1) == 1));
+    const int width = as_int(table.size(1));
+    const float scale = x[5] == Py_None ? (float)(1.0 / std::sqrt((double)c.D)) : float_arg(x[5]);
+    Tensor out, lse;
+    if (x[8] != Py_None) {
+      out = unpack(x[8]);
+      rows_tensor(out, at::kBFloat16, dev, dims);
+      plain(out.sizes() == q.sizes() && apart(out, c.k) && apart(out, c.v) &&
+            (apart(out, q) || (out.data_ptr() == q.data_ptr() && out.strides() == q.strides())));
+      one_place_each(out);
+    }
+    {
+      pybind11::gil_scoped_release no_gil;
+      const c10::DeviceGuard guard(dev);
+      if (x[8] == Py_None) out = at::empty(q.sizes(), q.options().requires_grad(false));
+      if (want_lse) lse = at::empty(q.sizes().slice(0, dims - 1), q.options().dtype(at::kFloat).requires_grad(false));
+      long long st[17];
+      int at = 0;
+      for (const Tensor* t : {&q, &static_cast<const Tensor&>(out)}) {
+        st[at++] = t->stride(0);
+        st[at++] = dims == 4 ? t->stride(1) : 0;
+        st[at++] = t->stride(dims - 2);
+      }
+      std::copy(c.strides, c.strides + 10, st + 6);
+      st[16] = table.stride(0);
+      const size_t need = abi.moonmath_gqa_decode_workspace(B, q_len, Hq, c.heads, c.D, c.page, width);
+      const Tensor ws = need ? bytes(need, q) : Tensor();
+      check_rc(abi.launch_gqa_decode_paged(q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), ptr_or_null(c.ks),
+                                           ptr_or_null(c.vs), out.data_ptr(), ptr_or_null(lse), lens.data_ptr(),
+                                           table.data_ptr(), B, q_len, Hq, c.heads, c.D, c.blocks, c.page, width, st,
+                                           scale, ptr_or_null(ws), stream_of(q)),
+               "launch_gqa_decode_paged");
+    }
+    PyObject* o = x[8];
+    if (o != Py_None)
+      Py_INCREF(o);
+    else
+      o = THPVariable_Wrap(out);
+    if (!want_lse) return o;
+    PyObject* pair = PyTuple_New(2);
+    if (!pair) return nullptr;
+    PyTuple_SET_ITEM(pair, 0, o);
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(lse));
+    return pair;
+  });
+}
+
+// q, k or None, positions, turns, axes (the caller's table), number of axes, layout, halves, inverse, inplace
+PyObject* rope(PyObject*, PyObject* const* x, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    plain(n == 10);
+    const Tensor &q = unpack(x[0]), &pos = unpack(x[2]), &turns = unpack(x[3]), &axes = unpack(x[4]);
+    const Tensor k = x[1] == Py_None ? Tensor() : unpack(x[1]);
+    const int A = int_arg(x[5]), bshd = layout_arg(x[6]);
+    const bool halves = bool_arg(x[7]), inverse = bool_arg(x[8]);
+    plain(x[9] == Py_False && q.is_cuda());  // in place: the wrapper sees that nothing is shared
+    check_modes();
+    const auto dev = q.device();
+    const int sax = bshd ? 1 : 2, hax = bshd ? 2 : 1;
+    rows_tensor(q, at::kBFloat16, dev, 4);
+    const int B = as_int(q.size(0)), S = as_int(q.size(sax)), D = as_int(q.size(3)), P = as_int(turns.numel());
+    plain((D == 64 || D == 128 || D == 256) && 2 * P <= D && q.size(hax) >= 1);
+    if (k.defined()) {
+      rows_tensor(k, at::kBFloat16, dev, 4);
+      plain(k.size(0) == B && k.size(sax) == S && k.size(3) == D && k.size(hax) >= 1);
+    }
+    plain(pos.scalar_type() == at::kInt && pos.layout() == at::kStrided && pos.device() == dev &&
+          !at::isTensorSubclassLike(pos) && !pos.is_neg());
+    const int64_t pd = pos.dim();
+    plain((pd == 2 || pd == 3) && pos.size(0) == A && pos.size(pd - 1) == S && (pd == 2 || pos.size(1) == B));
+    Tensor out[2];
+    {
+      pybind11::gil_scoped_release no_gil;
+      const c10::DeviceGuard guard(dev);
+      out[0] = at::empty(q.sizes(), q.options().requires_grad(false));
+      if (k.defined()) out[1] = at::empty(k.sizes(), k.options().requires_grad(false));
+      long long st[15] = {};
+      int at = 0;
+      for (const Tensor* t : {&q, &k, &static_cast<const Tensor&>(out[0]), &static_cast<const Tensor&>(out[1])})
+        for (int i : {0, sax, hax}) st[at++] = t->defined() ? t->stride(i) : 0;
+      st[12] = pos.stride(0);
+      st[13] = pd == 3 ? pos.stride(1) : 0;
+      st[14] = pos.stride(pd - 1);
+      check_rc(abi.launch_rope_axes(q.data_ptr(), ptr_or_null(k), out[0].data_ptr(), ptr_or_null(out[1]),
+                                    pos.data_ptr(), turns.data_ptr(), axes.data_ptr(), B, S, as_int(q.size(hax)),
+                                    k.defined() ? as_int(k.size(hax)) : 0, D, P, A, halves, inverse, st,
+                                    stream_of(q)),
+               "launch_rope_axes");
+    }
+    PyObject* pair = PyTuple_New(2);
+    if (!pair) return nullptr;
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(out[0]));
+    if (!k.defined()) Py_INCREF(Py_None);
+    PyTuple_SET_ITEM(pair, 1, k.defined() ? THPVariable_Wrap(out[1]) : Py_None);
+    return pair;
+  });
+}
+
 // bind({name: address}): the loaded library's launchers.
 PyObject* bind(PyObject*, PyObject* table) {
 #define MM_BIND(name)                                                            \
@@ -487,6 +768,10 @@ PyMethodDef methods[] = {MM_FAST(forward),
                          MM_FAST(mla_paged),
                          MM_FAST(mla_blocks),
                          MM_FAST(kv_quantize),
+                         MM_FAST(gqa_write),
+                         MM_FAST(gqa_read),
+                         MM_FAST(gqa_decode),
+                         MM_FAST(rope),
                          {"bind", bind, METH_O, nullptr},
                          {"bound_names", bound_names, METH_NOARGS, nullptr},
                          {"torch_version", torch_version, METH_NOARGS, nullptr},

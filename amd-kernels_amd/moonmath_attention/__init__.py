@@ -1,4 +1,5 @@
-"""MI355X (gfx950) bf16 flash-attention forward and fp8-KV absorbed-MLA decode.
+"""MI355X (gfx950) bf16 flash-attention forward, fp8-KV absorbed-MLA decode, and a
+paged K/V cache of grouped heads with its decode and rotary positions.
 
 Drop-in for the reference package's hot paths (moonmath reference
 moonmath_attention/__init__.py:11-31), backed by hand-written gfx950 HIP
@@ -10,6 +11,7 @@ kernels in ``libmoonmath_gfx950.so`` called through ctypes.
 """
 
 from ._kernel import forward, forward_lite
+from .gqa import gqa_decode_paged, gqa_kv_read, gqa_kv_write
 from .lite import LiteAttention
 from .mla import (
     mla_decode_a16w8,
@@ -23,6 +25,7 @@ from .mla import (
     mla_decode_a16w8_plan_parts_q,
     mla_kv_quantize,
 )
+from .rope import AxialRope
 
 __all__ = [
     "forward", "forward_lite", "LiteAttention",
@@ -31,4 +34,5 @@ __all__ = [
     "mla_decode_a16w8_plan_parts_q",
     "mla_decode_a16w8_multiq", "mla_decode_a16w8_multiq_paged_dev",
     "mla_decode_a16w8_multiq_plan_parts_q", "mla_kv_quantize",
+    "AxialRope", "gqa_decode_paged", "gqa_kv_read", "gqa_kv_write",
 ]

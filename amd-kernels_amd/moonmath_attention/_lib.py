@@ -22,6 +22,8 @@ _i = ctypes.c_int
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
 _ip = ctypes.POINTER(ctypes.c_int)
+_ll = ctypes.c_longlong
+_llp = ctypes.POINTER(_ll)
 
 # name -> (restype, argtypes)
 SIGNATURES = {}
@@ -67,6 +69,12 @@ SIGNATURES.update({
     "moonmath_fp8e4m3_to_bf16": (_i, [_p, _p, _i, _p]),
     "moonmath_pack_bf16": (_i, [_p, _p, _i, _i, _p]),
     "launch_mla_kv_quantize": (_i, [_p, _p, _p, _p, ctypes.c_longlong, ctypes.c_longlong, _f, _i, _p]),
+    "launch_gqa_kv_write": (_i, [_p, _p, _p, _p, _p, _p, _p, _ll, _i, _i, _i, _i, _llp, _p]),
+    "launch_gqa_kv_read": (_i, [_p, _p, _p, _p, _p, _p, _p, _ll, _i, _i, _i, _i, _llp, _p]),
+    "launch_gqa_decode_paged": (
+        _i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _llp, _f, _p, _p]),
+    "moonmath_gqa_decode_workspace": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
+    "launch_rope_axes": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _llp, _p]),
 })
 
 

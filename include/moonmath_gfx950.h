@@ -265,6 +265,63 @@ int moonmath_fp8e4m3_to_bf16(const void* in, void* out, int n, void* stream);
  * rules are the reference's bf16_round_one (csrc/attention_kernel.hip:110-145). */
 int moonmath_pack_bf16(const void* in, void* out, int n, int round_mode, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged K/V cache of grouped heads, and rotary positions of several axes. No
+ * counterparts in the reference. head_dim is 64, 128 or 256. Rows of head_dim
+ * elements are contiguous and lie on 16-byte boundaries; all other strides are
+ * the caller's, in elements, in one host array.
+ *
+ * A cache is a K and a V array of bf16 rows, or of e4m3fn rows with one fp32
+ * scale each (k_scale, v_scale; both NULL for bf16; 16-byte boundaries, a
+ * block's rows contiguous): 5 strides each, {block, head, row, scale block,
+ * scale head}. page: rows of a block, a power of two, at least 16.
+ * Codes: -2 head_dim, -3 heads, -4 sizes, -5 page or pairs, -6 null pointer,
+ * -8 grid overflow, -9 row stride above 2^26, -11 bad block-table or pool geometry.
+ * ------------------------------------------------------------------------- */
+
+/* Rows of new tokens into their slots (block * page + row; int32, outside
+ * [0, num_blocks * page): nothing written; equal slots in one call: parts of
+ * either token may stay). k, v: bf16 [n_tokens, Hkv, head_dim]. fp8: scale =
+ * max(amax of the row's finite values / 448, 2^-126), code = e4m3fn(x / scale) to
+ * nearest even, NaN where x is not finite. strides: k {token, head}, v {token,
+ * head}, then the two caches'. */
+int launch_gqa_kv_write(const void* k, const void* v, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                        const void* slots, long long n_tokens, int Hkv, int head_dim, int num_blocks, int page,
+                        const long long* strides, void* stream);
+
+/* Rows of slots back in bf16 (fp8: code * scale, to nearest even); zeros for a
+ * slot outside the pool. strides: as launch_gqa_kv_write. */
+int launch_gqa_kv_read(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
+                       const void* slots, void* k, void* v, long long n_tokens, int Hkv, int head_dim, int num_blocks,
+                       int page, const long long* strides, void* stream);
+
+/* Decode attention: query t of q_len (1..8) of request b attends its tokens
+ * [0, seq_lens[b] - q_len + t + 1), token i being row i % page of block
+ * block_table[b][i / page] (ids clamped to the pool, lengths to [0, max_blocks *
+ * page]); query head h reads kv head h / (Hq / Hkv). q, out: bf16 [B, q_len, Hq,
+ * head_dim] (out may be q); lse: fp32 [B, q_len, Hq] contiguous or NULL, ln of the
+ * softmax's sum. A query that sees no token: zeros, -inf. workspace:
+ * moonmath_gqa_decode_workspace bytes (NULL where that is 0), 16-byte aligned, its
+ * contents neither read nor kept across calls; calls that overlap need one each.
+ * strides: q {batch, query, head}, out {batch, query, head}, k cache, v cache,
+ * {block_table row}: 17. */
+int launch_gqa_decode_paged(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
+                            const void* v_scale, void* out, void* lse, const void* seq_lens, const void* block_table,
+                            int B, int q_len, int Hq, int Hkv, int head_dim, int num_blocks, int page, int max_blocks,
+                            const long long* strides, float scale, void* workspace, void* stream);
+size_t moonmath_gqa_decode_workspace(int B, int q_len, int Hq, int Hkv, int head_dim, int page, int max_blocks);
+
+/* Rotary positions: pair p of each head of q [B, S, Hq, head_dim] and k [B, S,
+ * Hk, head_dim] (Hk 0: q alone) turns by positions[axes[p]][b][s] * turns[p] of a
+ * full turn, inverse != 0: backwards. halves != 0: dims (p, n_pairs + p) are a
+ * pair, else (2p, 2p + 1); dims past 2 n_pairs pass through; n_pairs is a multiple
+ * of 8. positions int32, turns fp64 [n_pairs], axes int32 [n_pairs], on the
+ * device. q_out, k_out may be q, k. strides: q, k, q_out, k_out {batch, position,
+ * head} each, positions {axis, batch, position}: 15. */
+int launch_rope_axes(const void* q, const void* k, void* q_out, void* k_out, const void* positions, const void* turns,
+                     const void* axes, int B, int S, int Hq, int Hk, int head_dim, int n_pairs, int n_axes, int halves,
+                     int inverse, const long long* strides, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
