@@ -5,15 +5,15 @@
 //   o = sum_j softmax_j(scale * q . k_j) v_j   over the tokens j < S - q_len + t + 1,
 // zeros where that leaves no token, with lse = ln sum_j exp(scale * q . k_j).
 //
-// A task is one request, kv head and block of 16 * NT query rows (row t * G + g):
-// its rows share every K and V element read. The tasks' 128-token tiles, in order,
-// are cut into equal runs, one for each workgroup; a task that a cut divides leaves fp32
-// records (O, m, l) that a second kernel joins. So the work is even whatever the
-// lengths are, they are read on the device, and the workspace depends on neither.
+// A task is one request and RW "row sets" of 16 * NT query rows (row t * G + g of a kv
+// head): those of one kv head, or of neighbouring ones. The tasks' tiles of tokens, in
+// order, are cut into equal runs, one for each workgroup; a task that a cut divides
+// leaves fp32 records (O, m, l) that a second kernel joins. So the work is even whatever
+// the lengths are, they are read on the device, and the workspace depends on neither.
 //
-// Within a workgroup the four waves take 32-token steps of a tile in turn, each with
-// its own running maximum and sum (one pass over the data); they are joined in LDS
-// at the end of a task.
+// Within a workgroup RW waves take a row set each and the same tokens, and WAVES / RW
+// such groups of waves take the steps of 32 tokens in turn, each with its own running
+// maximum and sum (one pass over the data); they are joined in LDS at the task's end.
 //
 // No operand passes through LDS. 16x16x32 MFMAs compute S^T = K Q^T and
 // O^T = V^T P^T, so a lane keeps one query row (lane % 16) throughout:
@@ -32,11 +32,9 @@
 namespace mm {
 namespace gqa {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
-constexpr int kStep = 32;               // tokens of one wave's step
-constexpr int kTile = kStep * kWaves;   // tokens of one workgroup's tile
 constexpr int kMaxQLen = 8;
+constexpr int kMaxHeads = 1 << 16;
+constexpr long long kMaxTokens = (1LL << 31) - 64;  // of a request's table
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -47,14 +45,42 @@ struct DecodeArgs {
   float* lse;            // [B, q_len, Hq] contiguous, or null
   const int* seq_lens;   // [B]
   const int* table;      // [B, width] by table_s
-  float* rec_o;          // [2 * grid][16 * NT][D]
-  float* rec_ml;         // [2 * grid][16 * NT][2]
-  int4* joins;           // [grid]: the task that ends in this workgroup's run and began before it
+  float* rec_o;          // [2 * grid][16 * NT * RW][D]
+  float* rec_ml;         // [2 * grid][16 * NT * RW][2]
+  int4* joins;           // by task, or by run where there are more tasks than runs: what is to be joined
   long long q_s[3], out_s[3];  // batch, position, head; elements
   long long table_s;
-  int B, q_len, Hq, Hkv, G, rows, row_blocks;
+  int B, q_len, Hq, G, rows;   // rows = q_len * G
+  int sets;                    // row sets of one kv head that a task holds: RW, RW / 2 or RW / 4
+  int row_blocks, per;         // tasks of a kv head's rows, and of a request
+  int joins_by_task;
   int num_blocks, width, page_shift;
   float scale2;          // softmax scale * log2(e)
+  float inv_g;           // 1 / G
+};
+
+// Workgroups of a CU. One 16-row tile of up to 128 dims fits three waves a SIMD
+// (167 registers of 512); more rows or dims go one a SIMD: two would spill, or write
+// twice the records. 64 requests of 1K..8K tokens, 8 kv heads of 128: two 205 us, three
+// 194; 32 requests of windows of 4, 16 rows a position, 4 kv heads: two 92 us, one 80.
+constexpr int per_cu(int D, int nt) { return D * nt <= 128 ? 3 : 1; }
+
+// The kernel's shape: NT tiles of 16 rows for each wave, RW row sets; SHARED: of one
+// kv head, so that its rows are read by more than one wave.
+template <int D_, bool FP8_, int NT_, int RW_, bool SHARED_, bool SPLIT_>
+struct Shape {
+  static constexpr int D = D_, NT = NT_, RW = RW_;
+  static constexpr bool FP8 = FP8_, SPLIT = SPLIT_;
+  static constexpr int kWaves = !SPLIT && D * NT <= 128 ? 8 : 4, kThreads = 64 * kWaves;
+  static constexpr int kGroups = kWaves / RW;           // of waves, by tokens
+  static constexpr int kRow = FP8 ? D : 2 * D;          // bytes of a cached row
+  static constexpr int kStep = 32;                      // tokens of a wave's step
+  static constexpr int kTile = kStep * kGroups;         // tokens of a tile
+  static constexpr int kRows = 16 * NT * RW;            // of a task
+  static constexpr int kPerCu = SPLIT ? per_cu(D, NT) : 2;
+  static constexpr bool kOnce = !SHARED_ && SPLIT && !(D == 256 && !FP8);  // streamed past the caches
+  static constexpr int kKLoads = kRow / 64;             // 16-byte loads of K per lane and 16 tokens
+  static constexpr int kVWords = kRow / 64;             // dwords of V per lane and token
 };
 
 __device__ __forceinline__ float xor16_max(float x) {
@@ -72,63 +98,79 @@ __device__ __forceinline__ float xor16_sum(float x) {
 // the scalar cache, beside the waits of the vector loads.
 typedef const __attribute__((address_space(4))) int* ConstInts;
 
-__device__ __forceinline__ int clamped_len(const DecodeArgs& a, int b) {
+__device__ __forceinline__ int clamped(const DecodeArgs& a, int n) {
   const long long most = (long long)a.width << a.page_shift;
-  const int n = a.seq_lens[b];
   return n < 0 ? 0 : (n > most ? (int)most : n);
 }
-__device__ __forceinline__ int tiles_of(int len) { return (len >> 7) + ((len & 127) != 0); }
-static_assert(kTile == 128, "tiles_of counts 128-token tiles");
+__device__ __forceinline__ int len_of(const DecodeArgs& a, int b) { return clamped(a, ((ConstInts)(uintptr_t)a.seq_lens)[b]); }
+template <int TILE>
+__device__ __forceinline__ int tiles_of(int len) {
+  constexpr int kShift = __builtin_ctz(TILE);
+  static_assert(TILE == 1 << kShift, "tiles are powers of two");
+  return (len >> kShift) + ((len & (TILE - 1)) != 0);
+}
 
-// What one 32-token step of a wave reads: two 16-token halves, each within a page.
-template <int D, bool FP8>
+__device__ __forceinline__ long long uniform(long long x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+  return (long long)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// What one step of a wave reads, in halves of 16 tokens, each within a page.
+template <class C>
 struct Step {
-  static constexpr int kRow = FP8 ? D : 2 * D;        // bytes of a row
-  static constexpr int kKLoads = kRow / 64;           // 16-byte loads of K per lane and half
-  static constexpr int kVWords = kRow / 64;           // dwords of V per lane and token
-  u32x4 k[2][kKLoads];
-  uint32_t v[8][kVWords];
+  u32x4 k[2][C::kKLoads];
+  uint32_t v[8][C::kVWords];
   f32x4 ks[2], vs[2];
 };
 
-// The pages of a step's halves (wave-uniform, through the scalar cache).
+// The pages of a step's halves.
+template <class C>
 struct Pages {
   int id[2];
 };
-__device__ __forceinline__ Pages step_pages(const DecodeArgs& a, ConstInts row, int tok) {
-  Pages p;
+template <class C>
+__device__ __forceinline__ Pages<C> step_pages(const DecodeArgs& a, ConstInts row, int tok) {
+  Pages<C> p;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int at = min((tok + 16 * i) >> a.page_shift, a.width - 1);
-    const int id = row[at];
+    const int id = row[min((tok + 16 * i) >> a.page_shift, a.width - 1)];
     p.id[i] = min(max(id, 0), a.num_blocks - 1);
   }
   return p;
 }
 
-template <int D, bool FP8>
-__device__ __forceinline__ void load_k(const DecodeArgs& a, Step<D, FP8>& s, const Pages& pg, int tok, int head,
+// Streamed once: nothing of it is read again by this launch but the other half of a
+// line by the next load.
+template <class T, bool ONCE>
+__device__ __forceinline__ T stream(const char* p) {
+  if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+  return *reinterpret_cast<const T*>(p);
+}
+
+template <class C>
+__device__ __forceinline__ void load_k(const DecodeArgs& a, Step<C>& s, const Pages<C>& pg, int tok, int head,
                                        int lane) {
-  constexpr int kElem = FP8 ? 1 : 2;
+  constexpr int kElem = C::FP8 ? 1 : 2;
   const uint32_t off = (uint32_t)(lane & 15) * (uint32_t)(a.k.row_s * kElem) + 16u * (lane >> 4);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = (tok + 16 * i) & ((1 << a.page_shift) - 1);
     const char* kb = a.k.base + (pg.id[i] * a.k.block_s + head * a.k.head_s + row * a.k.row_s) * kElem;
 #pragma unroll
-    for (int c = 0; c < Step<D, FP8>::kKLoads; ++c) s.k[i][c] = *reinterpret_cast<const u32x4*>(kb + off + 64 * c);
-    if constexpr (FP8)
+    for (int c = 0; c < C::kKLoads; ++c) s.k[i][c] = stream<u32x4, C::kOnce>(kb + off + 64 * c);
+    if constexpr (C::FP8)
       s.ks[i] = *reinterpret_cast<const f32x4*>(a.k.scale + pg.id[i] * a.k.sblock_s + head * a.k.shead_s + row +
                                                 4 * (lane >> 4));
   }
 }
 
-template <int D, bool FP8>
-__device__ __forceinline__ void load_v(const DecodeArgs& a, Step<D, FP8>& s, const Pages& pg, int tok, int head,
+template <class C>
+__device__ __forceinline__ void load_v(const DecodeArgs& a, Step<C>& s, const Pages<C>& pg, int tok, int head,
                                        int lane) {
-  using S = Step<D, FP8>;
-  constexpr int kElem = FP8 ? 1 : 2;
-  const uint32_t off = 4u * (lane >> 4) * (uint32_t)(a.v.row_s * kElem) + (uint32_t)(S::kVWords * 4 * (lane & 15));
+  constexpr int kElem = C::FP8 ? 1 : 2;
+  const uint32_t off = 4u * (lane >> 4) * (uint32_t)(a.v.row_s * kElem) + (uint32_t)(C::kVWords * 4 * (lane & 15));
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = (tok + 16 * i) & ((1 << a.page_shift) - 1);
@@ -137,34 +179,34 @@ __device__ __forceinline__ void load_v(const DecodeArgs& a, Step<D, FP8>& s, con
     for (int r = 0; r < 4; ++r) {
       const char* p = vb + r * (a.v.row_s * kElem) + off;
       uint32_t* to = s.v[4 * i + r];
-      if constexpr (S::kVWords == 1) {
-        to[0] = *reinterpret_cast<const uint32_t*>(p);
-      } else if constexpr (S::kVWords == 2) {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+      if constexpr (C::kVWords == 1) {
+        to[0] = stream<uint32_t, C::kOnce>(p);
+      } else if constexpr (C::kVWords == 2) {
+        const u32x2 x = stream<u32x2, C::kOnce>(p);
         to[0] = x[0];
         to[1] = x[1];
       } else {
 #pragma unroll
-        for (int c = 0; c < S::kVWords / 4; ++c) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(p + 16 * c);
+        for (int c = 0; c < C::kVWords / 4; ++c) {
+          const u32x4 x = stream<u32x4, C::kOnce>(p + 16 * c);
 #pragma unroll
           for (int e = 0; e < 4; ++e) to[4 * c + e] = x[e];
         }
       }
     }
-    if constexpr (FP8)
+    if constexpr (C::FP8)
       s.vs[i] = *reinterpret_cast<const f32x4*>(a.v.scale + pg.id[i] * a.v.sblock_s + head * a.v.shead_s + row +
                                                 4 * (lane >> 4));
   }
 }
 
-// A wave's state: its query rows and what it has summed for them.
-template <int D, int NT>
+// A wave's query rows and what it has summed for them.
+template <class C>
 struct Rows {
-  bf16x8 q[NT][D / 32];
-  f32x4 o[NT][D / 16];   // o[nt][j][r]: row lane % 16, dim (D / 16) * (4 g + r) + j
-  float m[NT], l[NT];    // log2 domain; l over this lane's tokens only
-  int pos[NT];           // the row's query position
+  bf16x8 q[C::NT][C::D / 32];
+  f32x4 o[C::NT][C::D / 16];     // o[nt][j][r]: row lane % 16, dim (D / 16) * (4 g + r) + j
+  float m[C::NT], l[C::NT];      // log2 domain; l over this lane's tokens only
+  int pos[C::NT];                // the row's query position
 };
 
 // P is held as two bf16: its upper half and the rest, 2^-16 of it lost. The rest of a
@@ -178,21 +220,38 @@ __device__ __forceinline__ uint32_t zip(uint32_t even, uint32_t odd, bool hi) {
   return __builtin_amdgcn_perm(odd, even, hi ? 0x07060302u : 0x05040100u);
 }
 
-// O^T += V^T P^T for one step's 32 tokens. TAIL: tokens of `end` and above are
-// hidden from query position `only` and must not reach it even as 0 * NaN.
-template <int D, bool FP8, int NT, bool TAIL>
-__device__ __forceinline__ void add_pv(Rows<D, NT>& w, const Step<D, FP8>& s, const bf16x8 (&hi)[NT],
-                                       const bf16x8 (&lo)[NT], int tok0, int end, int only) {
-  using S = Step<D, FP8>;
-  constexpr int kPerWord = FP8 ? 4 : 2;  // elements of one dword of V
+// Whether V is finite in every token of [from, to) that the wave holds.
+template <class C>
+__device__ __forceinline__ bool finite_tail(const Step<C>& s, int tok0, int from, int to) {
+  constexpr uint32_t kOnes = C::FP8 ? 0x7F7F7F7Fu : 0x7F807F80u, kUnit = C::FP8 ? 0x01010101u : 0x00800080u,
+                     kTop = C::FP8 ? 0x80808080u : 0x80008000u;
+  uint32_t bad = 0;  // a field of ones carries into its top bit
 #pragma unroll
-  for (int c = 0; c < S::kVWords; ++c) {
+  for (int e = 0; e < 8; ++e) {
+    const int t = tok0 + (e & 3) + 16 * (e >> 2);
+    uint32_t any = 0;
+#pragma unroll
+    for (int c = 0; c < C::kVWords; ++c) any |= (s.v[e][c] & kOnes) + kUnit;
+    bad |= t >= from && t < to ? any & kTop : 0u;
+  }
+  return !__any(bad != 0);
+}
+
+// O^T += V^T P^T for the step's 32 tokens. TAIL: tokens of `end` and above are hidden from
+// query position `only` (-1: from all of them) and must not reach it even as 0 * NaN.
+template <class C, bool TAIL>
+__device__ __forceinline__ void add_pv(Rows<C>& w, const Step<C>& s, const bf16x8 (&hi)[C::NT],
+                                       const bf16x8 (&lo)[C::NT], int tok0, int end, int only) {
+  constexpr int kPerWord = C::FP8 ? 4 : 2;  // elements of one dword of V
+#pragma unroll
+  for (int c = 0; c < C::kVWords; ++c) {
+    if (c % (8 / kPerWord) == 0) sched_fence();
     uint32_t x[8][kPerWord / 2];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       uint32_t word = s.v[e][c];
       if constexpr (TAIL) word = tok0 + (e & 3) + 16 * (e >> 2) < end ? word : 0u;
-      if constexpr (FP8) {
+      if constexpr (C::FP8) {
         const u32x2 y = fp8x4_to_bf16(word);
         x[e][0] = y[0];
         x[e][1] = y[1];
@@ -208,12 +267,12 @@ __device__ __forceinline__ void add_pv(Rows<D, NT>& w, const Step<D, FP8>& s, co
       const bf16x8 vf = __builtin_bit_cast(bf16x8, f);
       const int j = c * kPerWord + h;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
+      for (int nt = 0; nt < C::NT; ++nt) {
         f32x4 acc = mfma16(vf, hi[nt], w.o[nt][j]);
         acc = mfma16(vf, lo[nt], acc);
         if constexpr (TAIL) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) w.o[nt][j][r] = w.pos[nt] == only ? acc[r] : w.o[nt][j][r];
+          for (int r = 0; r < 4; ++r) w.o[nt][j][r] = only < 0 || w.pos[nt] == only ? acc[r] : w.o[nt][j][r];
         } else {
           w.o[nt][j] = acc;
         }
@@ -222,25 +281,24 @@ __device__ __forceinline__ void add_pv(Rows<D, NT>& w, const Step<D, FP8>& s, co
   }
 }
 
-// One step's 32 tokens. Without TAIL every query position sees them all, and each
-// operand's registers take the next step's loads as soon as the products have read
-// them, so about a step (16 KB for 128 bf16 dims) is in flight for each wave at any time.
-template <int D, bool FP8, int NT, bool TAIL>
-__device__ __forceinline__ void compute_step(const DecodeArgs& a, Rows<D, NT>& w, Step<D, FP8>& s, int tok, int len,
-                                             const Pages& pg, int next, int head, int lane) {
-  using S = Step<D, FP8>;
-  const int tok0 = tok + 4 * (lane >> 4);  // this lane's tokens: tok0 + r and tok0 + 16 + r
-  bf16x8 hi[NT], lo[NT];
-  f32x4 sc[NT][2];
+// One step. Without TAIL every query position sees all its tokens, and each operand's
+// registers take the next step's loads as soon as the products have read them, so
+// about a step (16 KB) is in flight for each wave at any time.
+template <class C, bool TAIL>
+__device__ __forceinline__ void compute_step(const DecodeArgs& a, Rows<C>& w, Step<C>& s, int tok, int len,
+                                             const Pages<C>& pg, int next, int head, int lane) {
+  const int tok0 = tok + 4 * (lane >> 4);  // this lane's tokens: tok0 + 16 i + r
+  f32x4 sc[C::NT][2];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+  for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
     for (int i = 0; i < 2; ++i) sc[nt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
+    if (C::FP8) sched_fence();
 #pragma unroll
-    for (int c = 0; c < S::kKLoads; ++c) {
-      if constexpr (FP8) {
+    for (int c = 0; c < C::kKLoads; ++c) {
+      if constexpr (C::FP8) {
         // 16 dims of a load feed two MFMAs: Q is laid out to match.
         bf16x8 kf[2];
 #pragma unroll
@@ -249,21 +307,27 @@ __device__ __forceinline__ void compute_step(const DecodeArgs& a, Rows<D, NT>& w
           kf[h] = __builtin_bit_cast(bf16x8, u32x4{x[0], x[1], y[0], y[1]});
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < C::NT; ++nt) {
           sc[nt][i] = mfma16(kf[0], w.q[nt][2 * c], sc[nt][i]);
           sc[nt][i] = mfma16(kf[1], w.q[nt][2 * c + 1], sc[nt][i]);
         }
       } else {
         const bf16x8 kf = __builtin_bit_cast(bf16x8, s.k[i][c]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt][i] = mfma16(kf, w.q[nt][c], sc[nt][i]);
+        for (int nt = 0; nt < C::NT; ++nt) sc[nt][i] = mfma16(kf, w.q[nt][c], sc[nt][i]);
       }
     }
   }
-  const f32x4 ks[2] = {s.ks[0], s.ks[1]};
-  if constexpr (!TAIL) load_k<D, FP8>(a, s, pg, next, head, lane);
+  f32x4 ks[2];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
+  for (int i = 0; i < 2; ++i) ks[i] = s.ks[i];
+  if constexpr (!TAIL) {
+    sched_fence();
+    load_k<C>(a, s, pg, next, head, lane);
+    sched_fence();
+  }
+#pragma unroll
+  for (int nt = 0; nt < C::NT; ++nt) {
     const int end = len - a.q_len + w.pos[nt] + 1;  // the row sees the tokens before it
     float mx = w.m[nt];
 #pragma unroll
@@ -271,7 +335,7 @@ __device__ __forceinline__ void compute_step(const DecodeArgs& a, Rows<D, NT>& w
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         float x = sc[nt][i][r] * a.scale2;
-        if constexpr (FP8) x *= ks[i][r];
+        if constexpr (C::FP8) x *= ks[i][r];
         if constexpr (TAIL) x = tok0 + 16 * i + r < end ? x : -__builtin_inff();
         sc[nt][i][r] = x;
         mx = fmaxf(mx, x);
@@ -282,19 +346,27 @@ __device__ __forceinline__ void compute_step(const DecodeArgs& a, Rows<D, NT>& w
       const float f = __builtin_amdgcn_exp2f(w.m[nt] - mx);
       w.l[nt] *= f;
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j)
+      for (int j = 0; j < C::D / 16; ++j)
 #pragma unroll
         for (int r = 0; r < 4; ++r) w.o[nt][j][r] *= f;
       w.m[nt] = mx;
     }
+  }
+  bool apiece = false;  // query positions see different numbers of these tokens, and not all V is finite
+  if constexpr (TAIL) apiece = !finite_tail<C>(s, tok0, len - a.q_len + 1, len);
+  sched_fence();
+  bf16x8 hi[C::NT], lo[C::NT];
+#pragma unroll
+  for (int nt = 0; nt < C::NT; ++nt) {
+    const int end = len - a.q_len + w.pos[nt] + 1;
     float p[8], sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        float x = __builtin_amdgcn_exp2f(sc[nt][i][r] - mx);
+        float x = __builtin_amdgcn_exp2f(sc[nt][i][r] - w.m[nt]);
         sum += x;
-        if constexpr (FP8) x *= s.vs[i][r];
+        if constexpr (C::FP8) x *= s.vs[i][r];
         if constexpr (TAIL) x = tok0 + 16 * i + r < end ? x : 0.f;  // a hidden row's scale may be NaN
         p[4 * i + r] = x;
       }
@@ -308,19 +380,13 @@ __device__ __forceinline__ void compute_step(const DecodeArgs& a, Rows<D, NT>& w
     hi[nt] = __builtin_bit_cast(bf16x8, h);
     lo[nt] = __builtin_bit_cast(bf16x8, l);
   }
-  if constexpr (TAIL) {
-    // Query positions see different numbers of these tokens: each adds its own.
-    for (int t = 0; t < a.q_len; ++t) add_pv<D, FP8, NT, true>(w, s, hi, lo, tok0, len - a.q_len + t + 1, t);
-  } else {
-    add_pv<D, FP8, NT, false>(w, s, hi, lo, tok0, 0, 0);
-    load_v<D, FP8>(a, s, pg, next, head, lane);
+  if constexpr (!TAIL) {
+    add_pv<C, false>(w, s, hi, lo, tok0, 0, 0);
+  } else {  // a hidden token weighs 0, which suffices where V is finite; one past the end is taken as 0
+    for (int t = apiece ? 0 : a.q_len - 1; t < a.q_len; ++t)
+      add_pv<C, true>(w, s, hi, lo, tok0, len - a.q_len + t + 1, apiece ? t : -1);
   }
-}
-
-__device__ __forceinline__ long long uniform(long long x) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
-  return (long long)((uint64_t)hi << 32 | lo);
+  if constexpr (!TAIL) load_v<C>(a, s, pg, next, head, lane);
 }
 
 // The runs: tile i of `total` belongs to run w where start(w) <= i < start(w + 1),
@@ -330,124 +396,138 @@ __device__ __forceinline__ long long run_start(long long total, int runs, int w)
 }
 
 // A workgroup's run, and the request in which its first tile lies with the number
-// of tiles before that. Every thread calls it.
+// of tiles before that.
 struct Run {
   long long total;
   long long start, end;   // tiles of all tasks, in order
   long long before;       // tiles before request b
   int runs, b;
 };
-__device__ Run find_run(const DecodeArgs& a, int wg, int grid, long long* sh) {
+// Every thread calls it. Requests are taken THREADS at a time, one for each thread, and
+// a prefix sum finds the one that holds the run's first tile.
+template <int THREADS, int TILE>
+__device__ Run find_run(const DecodeArgs& a, int wg, int grid) {
+  constexpr int kWaves = THREADS / 64;
+  __shared__ int sh_sum[2][kWaves];
+  __shared__ long long sh_found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per = a.Hkv * a.row_blocks;
-  long long mine = 0;
-  for (int b = tid; b < a.B; b += kThreads) mine += (long long)tiles_of(clamped_len(a, b));
+  // A wave's 64 requests have fewer than 2^32 tiles; sums over waves are 64 bits.
+  static_assert(TILE >= 32, "64 requests of at most kMaxTokens");
+  const auto group = [&](int b0, int turn, int& n, int& incl, long long& ahead, long long& sum) {
+    n = b0 + tid < a.B ? tiles_of<TILE>(clamped(a, a.seq_lens[b0 + tid])) : 0;
+    incl = wave_incl_scan(n);
+    if (lane == 63) sh_sum[turn][wave] = incl;
+    __syncthreads();
+    ahead = sum = 0;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) mine += __shfl_xor(mine, d);
-  if (lane == 0) sh[wave] = mine;
-  __syncthreads();
-  long long total = 0;
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) total += sh[i];
-  __syncthreads();
-  Run run;
-  run.total = total = uniform(total * per);
+    for (int i = 0; i < kWaves; ++i) {
+      if (i < wave) ahead += (uint32_t)sh_sum[turn][i];
+      sum += (uint32_t)sh_sum[turn][i];
+    }
+  };
+  int n, incl;
+  long long ahead, sum, total = 0;
+  for (int b0 = 0, turn = 0; b0 < a.B; b0 += THREADS, turn ^= 1) {
+    group(b0, turn, n, incl, ahead, sum);
+    total += sum;
+  }
+  Run run{};
+  run.total = total = uniform(total * a.per);
   run.runs = (int)min((long long)grid, total);
-  run.start = run.end = run.before = 0;
   run.b = a.B;
   if (wg >= run.runs) return run;
   run.start = run_start(total, run.runs, wg);
   run.end = run_start(total, run.runs, wg + 1);
-  // Requests in groups of 256: a prefix sum finds the one that holds `start`.
   long long base = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-    const int b = b0 + tid;
-    const long long n = b < a.B ? (long long)tiles_of(clamped_len(a, b)) * per : 0;
-    long long incl = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const long long x = __shfl_up(incl, d);
-      if (lane >= d) incl += x;
-    }
-    if (lane == 63) sh[wave] = incl;
-    __syncthreads();
-    long long ahead = base, sum = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      if (i < wave) ahead += sh[i];
-      sum += sh[i];
-    }
-    if (n > 0 && run.start >= ahead + incl - n && run.start < ahead + incl) {
-      sh[kWaves] = b;
-      sh[kWaves + 1] = ahead + incl - n;
-    }
-    __syncthreads();
-    if (run.start < base + sum) {
-      run.b = __builtin_amdgcn_readfirstlane((int)sh[kWaves]);
-      run.before = uniform(sh[kWaves + 1]);
+  for (int b0 = 0, turn = 0; b0 < a.B; b0 += THREADS, turn ^= 1) {
+    if (a.B > THREADS) {
       __syncthreads();
-      return run;
+      group(b0, turn, n, incl, ahead, sum);
+    }
+    const long long before = (base + ahead + (uint32_t)incl - (uint32_t)n) * a.per;
+    if (run.start >= before && run.start < before + (long long)n * a.per) {
+      sh_found[0] = b0 + tid;
+      sh_found[1] = before;
     }
     base += sum;
-    __syncthreads();
+    if (run.start < base * a.per) break;
   }
+  __syncthreads();
+  run.b = uniform((int)sh_found[0]);
+  run.before = uniform(sh_found[1]);
   return run;
 }
 
-// Workgroups of a CU: as many as the registers of their waves allow (512 of a SIMD).
-template <int D, int NT>
-constexpr int kPerCu = D * NT <= 128 ? 2 : 1;
+// Row `row` of a task: kv head, and row of that head's q_len * G (it may be past them).
+template <int NT>
+__device__ __forceinline__ void row_of(const DecodeArgs& a, int head0, int block, int row, int& head, int& r) {
+  const int set = row / (16 * NT), in_head = a.sets == 1 ? set : a.sets == 2 ? set >> 1 : set >> 2;
+  head = head0 + in_head;
+  r = (block * a.sets + (set & (a.sets - 1))) * 16 * NT + row % (16 * NT);
+}
+// r / G for r below q_len * G: exact, as (r + 1/2) / G lies 1 / (2 G) from a whole number.
+__device__ __forceinline__ int position(const DecodeArgs& a, int r) { return (int)(((float)r + 0.5f) * a.inv_g); }
 
-template <int D, bool FP8, int NT>
-__global__ __launch_bounds__(kThreads, (kPerCu<D, NT>)) void gqa_decode_kernel(const DecodeArgs a, const int split) {
-  constexpr int kRows = 16 * NT;
+// SPLIT: the workgroup takes its run of all tasks' tiles. Otherwise a whole task:
+// nothing is planned, and the first step is loaded before the request's length is there.
+template <class C>
+__global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(const DecodeArgs a) {
+  constexpr int D = C::D, NT = C::NT, kWaves = C::kWaves, kThreads = C::kThreads;
+  constexpr bool SPLIT = C::SPLIT;
   constexpr int kPitch = D + 4;  // floats: rows of the join start on different banks
   __shared__ float sh_o[kWaves][16][kPitch];
-  __shared__ float sh_ml[kWaves][kRows][2];
-  __shared__ long long sh_plan[kWaves + 2];
+  __shared__ float sh_ml[C::kGroups][C::kRows][2];
 
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int grid = gridDim.x;
-  const int wg = xcd_remap(blockIdx.x, grid);
-  const int per = a.Hkv * a.row_blocks;
+  const int wave = uniform(tid >> 6), rw = wave % C::RW, tg = wave / C::RW;
 
+  int wg = 0, b, task = 0, grid = 0;
   Run run{};
-  if (split) {
-    run = find_run(a, wg, grid, sh_plan);
-    if (tid == 0) a.joins[wg] = int4{-1, 0, 0, 0};
-  } else {  // a whole task for each workgroup
-    run.b = wg / per;
-    const int n = tiles_of(clamped_len(a, run.b));
-    run.before = 0;
-    run.start = (long long)(wg % per) * n;
-    run.end = run.start + n;
+  if constexpr (SPLIT) {
+    grid = gridDim.x;
+    wg = xcd_remap(blockIdx.x, grid);
+    run = find_run<kThreads, C::kTile>(a, wg, grid);
+    if (!a.joins_by_task && tid == 0) a.joins[wg] = int4{-1, 0, 0, 0};
+    b = run.b;
+  } else {
+    b = blockIdx.x;
+    task = blockIdx.y;
+    run.end = 1;
   }
   bool first = true;
-  int b = run.b;
   long long at = run.start, before = run.before;
   while (at < run.end && b < a.B) {
-    const int len = __builtin_amdgcn_readfirstlane(clamped_len(a, b));
-    const int tiles = tiles_of(len);
-    if (at - before >= (long long)tiles * per) {  // done with request b
-      before += (long long)tiles * per;
-      ++b;
-      continue;
+    int len = 0, tiles = 0, tile0 = 0, tile1 = 0;
+    if constexpr (SPLIT) {
+      len = len_of(a, b);
+      tiles = tiles_of<C::kTile>(len);
+      if (at - before >= (long long)tiles * a.per) {  // done with request b
+        before += (long long)tiles * a.per;
+        ++b;
+        continue;
+      }
+      task = uniform((int)((at - before) / tiles));
+      tile0 = uniform((int)((at - before) - (long long)task * tiles));
+      tile1 = uniform((int)min((long long)tiles, tile0 + (run.end - at)));
     }
-    const int task = __builtin_amdgcn_readfirstlane((int)((at - before) / tiles));
-    const int tile0 = __builtin_amdgcn_readfirstlane((int)((at - before) - (long long)task * tiles));
-    const int tile1 = __builtin_amdgcn_readfirstlane((int)min((long long)tiles, tile0 + (run.end - at)));
-    const int head = task / a.row_blocks, row0 = (task % a.row_blocks) * kRows;
-    const int rows = min(kRows, a.rows - row0);
+    const int group = a.row_blocks == 1 ? task : task / a.row_blocks;
+    const int block = a.row_blocks == 1 ? 0 : task - group * a.row_blocks;
+    const int head0 = a.sets == C::RW ? group : a.sets * 2 == C::RW ? group * 2 : group * 4;
     const ConstInts table = (ConstInts)(uintptr_t)(a.table + (long long)b * a.table_s);
 
-    Rows<D, NT> w;
+    // This wave's first step, and its query rows.
+    int st = tile0 * C::kGroups + tg;
+    Step<C> s;
+    Pages<C> pg = step_pages<C>(a, table, st * C::kStep);
+    Rows<C> w;
     const int n = lane & 15, g = lane >> 4;
+    int head, row0;
+    row_of<NT>(a, head0, block, rw * 16 * NT, head, row0);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = row0 + 16 * nt + n;
-      const bool live = 16 * nt + n < rows;
-      const int t = live ? r / a.G : a.q_len - 1;
+      const bool live = r < a.rows;
+      const int t = live ? position(a, r) : a.q_len - 1;
       w.pos[nt] = t;
       w.m[nt] = kNegFltMax;
       w.l[nt] = 0.f;
@@ -457,200 +537,236 @@ __global__ __launch_bounds__(kThreads, (kPerCu<D, NT>)) void gqa_decode_kernel(c
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         // dims of MFMA c for lane group g, as K's loads have them
-        const int d = FP8 ? 64 * (c / 2) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g;
+        const int d = C::FP8 ? 64 * (c / 2) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g;
         u32x4 x = *reinterpret_cast<const u32x4*>(qr + 2 * d);
         if (!live) x = u32x4{0u, 0u, 0u, 0u};
         w.q[nt][c] = __builtin_bit_cast(bf16x8, x);
       }
     }
+    // K before V here as in the loop: the compiler's wait for K there counts the loads
+    // that may have been issued since on every way into it.
+    sched_fence();
+    load_k<C>(a, s, pg, st * C::kStep, head, lane);
+    sched_fence();
+    load_v<C>(a, s, pg, st * C::kStep, head, lane);
+    if constexpr (!SPLIT) {
+      len = len_of(a, b);
+      tile1 = tiles = tiles_of<C::kTile>(len);
+    }
 
-    // This wave's steps: every fourth one. Only the last can hold a token that some
-    // position does not see (q_len - 1 + 31 tokens lie in two steps at most, of two
-    // waves). Loads past the last step repeat it: one under a branch would make the
-    // compiler wait for all of them.
-    int st = tile0 * kWaves + wave;
-    const int s_end = min(tile1 * kWaves, (len + kStep - 1) / kStep);
-    if (st < s_end) {
-      const int s_last = st + (s_end - 1 - st) / kWaves * kWaves;
-      const int s_full = (len - a.q_len + 1) >> 5;  // steps before it are seen by all
-      static_assert(kStep == 32, "s_full counts 32-token steps");
-      Step<D, FP8> s;
-      Pages pg = step_pages(a, table, st * kStep);
-      load_k<D, FP8>(a, s, pg, st * kStep, head, lane);
-      load_v<D, FP8>(a, s, pg, st * kStep, head, lane);
-      int next = min(st + kWaves, s_last);
-      pg = step_pages(a, table, next * kStep);
-      for (; st <= s_last && st < s_full; st += kWaves) {
-        const int after = min(next + kWaves, s_last);
-        const Pages pa = step_pages(a, table, after * kStep);
-        compute_step<D, FP8, NT, false>(a, w, s, st * kStep, len, pg, next * kStep, head, lane);
+    // Its steps are every kGroups-th one. Those from s_full on hold tokens that some
+    // position does not see: a step's worth and q_len - 1, in two steps at most. Loads
+    // past the last step repeat it: one under a branch would make the compiler wait
+    // for all of them.
+    const int s_end = min(tile1 * C::kGroups, tiles_of<C::kStep>(len));
+    if (st < s_end && row0 < a.rows) {
+      const int s_last = st + (s_end - 1 - st) / C::kGroups * C::kGroups;
+      const int seen = len - a.q_len + 1;
+      const int s_full = seen > 0 ? seen / C::kStep : 0;
+      int next = min(st + C::kGroups, s_last);
+      pg = step_pages<C>(a, table, next * C::kStep);
+      for (; st <= s_last && st < s_full; st += C::kGroups) {
+        const int after = min(next + C::kGroups, s_last);
+        const Pages<C> pa = step_pages<C>(a, table, after * C::kStep);
+        compute_step<C, false>(a, w, s, st * C::kStep, len, pg, next * C::kStep, head, lane);
         pg = pa;
         next = after;
       }
-      if (st <= s_last) compute_step<D, FP8, NT, true>(a, w, s, st * kStep, len, pg, 0, head, lane);
+      while (st <= s_last) {
+        compute_step<C, true>(a, w, s, st * C::kStep, len, pg, 0, head, lane);
+        st += C::kGroups;
+        if (C::kGroups > 1 || st > s_last) break;  // a wave of several has one such step
+        pg = step_pages<C>(a, table, st * C::kStep);
+        load_k<C>(a, s, pg, st * C::kStep, head, lane);
+        load_v<C>(a, s, pg, st * C::kStep, head, lane);
+      }
     }
 
     // Join the waves.
-    const bool whole = tile0 == 0 && tile1 == tiles;
+    const bool whole = !SPLIT || (tile0 == 0 && tile1 == tiles);
     const int rec = 2 * wg + (first ? 0 : 1);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       w.l[nt] = xor32_sum(xor16_sum(w.l[nt]));
       if (g == 0) {
-        sh_ml[wave][16 * nt + n][0] = w.m[nt];
-        sh_ml[wave][16 * nt + n][1] = w.l[nt];
+        sh_ml[tg][(rw * NT + nt) * 16 + n][0] = w.m[nt];
+        sh_ml[tg][(rw * NT + nt) * 16 + n][1] = w.l[nt];
       }
     }
     __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      if (16 * nt < rows) {
-        {
-          float top = sh_ml[0][16 * nt + n][0];
+      {
+        const int row = (rw * NT + nt) * 16 + n;
+        float top = sh_ml[0][row][0];
 #pragma unroll
-          for (int i = 1; i < kWaves; ++i) top = fmaxf(top, sh_ml[i][16 * nt + n][0]);
-          const float f = __builtin_amdgcn_exp2f(w.m[nt] - top);
-          // A lane's dims (D / 16) * 4 g .. + D / 4 of its row, in order.
-          float* to = &sh_o[wave][n][D / 4 * g];
+        for (int i = 1; i < C::kGroups; ++i) top = fmaxf(top, sh_ml[i][row][0]);
+        const float f = __builtin_amdgcn_exp2f(w.m[nt] - top);
+        // A lane's dims (D / 16) * 4 g .. + D / 4 of its row, in order.
+        float* to = &sh_o[wave][n][D / 4 * g];
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int j = 0; j < D / 16; j += 4)
-              *reinterpret_cast<f32x4*>(to + (D / 16) * r + j) =
-                  f32x4{w.o[nt][j][r] * f, w.o[nt][j + 1][r] * f, w.o[nt][j + 2][r] * f, w.o[nt][j + 3][r] * f};
-        }
-        __syncthreads();
-        {
-          // 16 threads for each row, D / 16 dims each.
-          constexpr int kPer = D / 16;
-          const int r = tid >> 4, d0 = (tid & 15) * kPer, row = 16 * nt + r;
-          if (row < rows) {
-            float top = sh_ml[0][row][0];
+          for (int j = 0; j < D / 16; j += 4)
+            *reinterpret_cast<f32x4*>(to + (D / 16) * r + j) =
+                f32x4{w.o[nt][j][r] * f, w.o[nt][j + 1][r] * f, w.o[nt][j + 2][r] * f, w.o[nt][j + 3][r] * f};
+      }
+      __syncthreads();
+      {
+        // The row sets' tiles nt: kAcross threads for each of 16 * RW rows, kPer dims each.
+        constexpr int kAcross = kThreads / (16 * C::RW), kPer = D / kAcross;
+        const int set = tid / (16 * kAcross), in = tid / kAcross % 16, d0 = tid % kAcross * kPer;
+        const int row = (set * NT + nt) * 16 + in;
+        int h, R;
+        row_of<NT>(a, head0, block, row, h, R);
+        if (R < a.rows) {
+          float top = sh_ml[0][row][0];
 #pragma unroll
-            for (int i = 1; i < kWaves; ++i) top = fmaxf(top, sh_ml[i][row][0]);
-            float l = 0.f;
+          for (int i = 1; i < C::kGroups; ++i) top = fmaxf(top, sh_ml[i][row][0]);
+          float l = 0.f;
 #pragma unroll
-            for (int i = 0; i < kWaves; ++i) l += sh_ml[i][row][1] * __builtin_amdgcn_exp2f(sh_ml[i][row][0] - top);
-            float o[kPer];
+          for (int i = 0; i < C::kGroups; ++i) l += sh_ml[i][row][1] * __builtin_amdgcn_exp2f(sh_ml[i][row][0] - top);
+          float o[kPer];
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-              o[j] = 0.f;
+          for (int j = 0; j < kPer; ++j) {
+            o[j] = 0.f;
 #pragma unroll
-              for (int i = 0; i < kWaves; ++i) o[j] += sh_o[i][r][d0 + j];
-            }
-            if (whole) {
-              const int R = row0 + row, t = R / a.G, h = head * a.G + R - t * a.G;
-              const bool none = len - a.q_len + t + 1 <= 0;  // the row sees no token
-              const float inv = 1.f / l;
-              char* to = a.out + 2 * (b * a.out_s[0] + t * a.out_s[1] + h * a.out_s[2] + d0);
+            for (int i = 0; i < C::kGroups; ++i) o[j] += sh_o[i * C::RW + set][in][d0 + j];
+          }
+          if (whole) {
+            const int t = position(a, R), hq = h * a.G + R - t * a.G;
+            const bool none = len - a.q_len + t + 1 <= 0;  // the row sees no token
+            const float inv = 1.f / l;
+            char* to = a.out + 2 * (b * a.out_s[0] + t * a.out_s[1] + hq * a.out_s[2] + d0);
 #pragma unroll
-              for (int j = 0; j < kPer; j += 4) {
-                u32x2 x;
-                x[0] = pack2_bf16_canon<kRTNE>(o[j] * inv, o[j + 1] * inv);
-                x[1] = pack2_bf16_canon<kRTNE>(o[j + 2] * inv, o[j + 3] * inv);
-                if (none) x = u32x2{0u, 0u};
-                *reinterpret_cast<u32x2*>(to + 2 * j) = x;
-              }
-              if (a.lse && (tid & 15) == 0)
-                a.lse[((long long)b * a.q_len + t) * a.Hq + h] =
-                    none ? -__builtin_inff() : kLn2 * (top + __builtin_amdgcn_logf(l));
-            } else {
-              float* to = a.rec_o + ((long long)rec * kRows + row) * D + d0;
+            for (int j = 0; j < kPer; j += 2)
+              *reinterpret_cast<uint32_t*>(to + 2 * j) =
+                  none ? 0u : pack2_bf16_canon<kRTNE>(o[j] * inv, o[j + 1] * inv);
+            if (a.lse && d0 == 0)
+              a.lse[((long long)b * a.q_len + t) * a.Hq + hq] =
+                  none ? -__builtin_inff() : kLn2 * (top + __builtin_amdgcn_logf(l));
+          } else {
+            float* to = a.rec_o + ((long long)rec * C::kRows + row) * D + d0;
 #pragma unroll
-              for (int j = 0; j < kPer; j += 4)
-                *reinterpret_cast<f32x4*>(to + j) = f32x4{o[j], o[j + 1], o[j + 2], o[j + 3]};
-              if ((tid & 15) == 0) {
-                a.rec_ml[((long long)rec * kRows + row) * 2] = top;
-                a.rec_ml[((long long)rec * kRows + row) * 2 + 1] = l;
-              }
+            for (int j = 0; j < kPer; ++j) to[j] = o[j];
+            if (d0 == 0) {
+              a.rec_ml[((long long)rec * C::kRows + row) * 2] = top;
+              a.rec_ml[((long long)rec * C::kRows + row) * 2 + 1] = l;
             }
           }
         }
-        __syncthreads();
       }
+      __syncthreads();
     }
-    if (!whole && tile1 == tiles && tid == 0) {
-      // The task ends here and began in an earlier run: that run, and which of its
-      // two records holds it (the first segment's, or the last's).
-      const long long began = before + (long long)task * tiles;
-      int w0 = (int)(began * run.runs / run.total);
-      while (run_start(run.total, run.runs, w0) > began) --w0;
-      while (run_start(run.total, run.runs, w0 + 1) <= began) ++w0;
-      a.joins[wg] = int4{b, task, w0, run_start(run.total, run.runs, w0) == began ? 0 : 1};
+    if constexpr (!SPLIT) return;
+    if (tile1 == tiles && tid == 0) {
+      // The task ends in this run. Where it began in an earlier one: that run, and which
+      // of its two records holds the beginning (its first segment's, or its last's).
+      int4 join{-1, 0, 0, 0};
+      if (!whole) {
+        const long long began = before + (long long)task * tiles;
+        int w0 = (int)(began * run.runs / run.total);
+        while (run_start(run.total, run.runs, w0) > began) --w0;
+        while (run_start(run.total, run.runs, w0 + 1) <= began) ++w0;
+        join = int4{b, task, 2 * w0 + (run_start(run.total, run.runs, w0) == began ? 0 : 1), wg};
+      }
+      if (a.joins_by_task)
+        a.joins[b * a.per + task] = join;
+      else if (!whole)
+        a.joins[wg] = join;  // of the first segment only: one for each run
     }
     first = false;
     at += tile1 - tile0;
   }
 
   // Requests without a token: zeros.
-  const int step = split ? grid : 1;
-  for (int e = split ? wg : wg / per; e < a.B; e += step) {
-    if (clamped_len(a, e) == 0) {
-      const int lo = split ? 0 : wg % per, hi = split ? per : lo + 1;
-      for (int task = lo; task < hi; ++task) {
-        const int head = task / a.row_blocks, row0 = (task % a.row_blocks) * kRows;
-        const int rows = min(kRows, a.rows - row0);
-        for (int i = tid; i < rows * (D / 8); i += kThreads) {
-          const int R = row0 + i / (D / 8), t = R / a.G, h = head * a.G + R - t * a.G;
-          *reinterpret_cast<u32x4*>(a.out + 2 * (e * a.out_s[0] + t * a.out_s[1] + h * a.out_s[2] + 8 * (i % (D / 8)))) =
-              u32x4{0u, 0u, 0u, 0u};
-          if (a.lse && i % (D / 8) == 0) a.lse[((long long)e * a.q_len + t) * a.Hq + h] = -__builtin_inff();
-        }
-      }
+  for (int e = wg; SPLIT && e < a.B; e += grid) {
+    if (len_of(a, e) != 0) continue;
+    for (int i = tid; i < a.q_len * a.Hq * (D / 8); i += kThreads) {
+      const int th = i / (D / 8), t = th / a.Hq, h = th - t * a.Hq;
+      *reinterpret_cast<u32x4*>(a.out + 2 * (e * a.out_s[0] + t * a.out_s[1] + h * a.out_s[2] + 8 * (i % (D / 8)))) =
+          u32x4{0u, 0u, 0u, 0u};
+      if (a.lse && i % (D / 8) == 0) a.lse[(long long)e * a.q_len * a.Hq + th] = -__builtin_inff();
     }
-    if (!split) break;
+    if (a.joins_by_task)
+      for (int i = tid; i < a.per; i += kThreads) a.joins[e * a.per + i] = int4{-1, 0, 0, 0};
   }
 }
 
-// Joins the records of a task that several runs hold: rows of O and (m, l), summed in
-// the order of the runs. Launched for every run; one that ends no such task
-// returns. PER_ROW waves share a row's records.
-template <int D, int NT, int PER_ROW>
-__global__ __launch_bounds__(kThreads) void gqa_join_kernel(const DecodeArgs a) {
-  constexpr int kRows = 16 * NT, kPer = D / 64;
-  __shared__ float sh[PER_ROW > 1 ? PER_ROW : 1][D];
-  const int wg = blockIdx.x;
-  const int4 j = a.joins[wg];
+// Joins the records of a task that several runs hold: rows of O and (m, l), in an order
+// that the call's shape and lengths alone decide. PER_ROW of a workgroup's 16 waves
+// share a row's records, each with a running maximum over its own, four loaded at once.
+template <int D, int NT, int RW, int PER_ROW>
+__global__ __launch_bounds__(1024) void gqa_join_kernel(const DecodeArgs a) {
+  constexpr int kRows = 16 * NT * RW, kPer = D / 64;
+  __shared__ float sh_o[PER_ROW > 1 ? 16 : 1][D];
+  __shared__ float sh_ml[16][2];
+  const int4 j = a.joins[blockIdx.x];
   if (j.x < 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int head = j.y / a.row_blocks, row0 = (j.y % a.row_blocks) * kRows;
-  const int row = blockIdx.y * (kWaves / PER_ROW) + wave / PER_ROW;
-  if (row >= min(kRows, a.rows - row0)) return;
-  const int n = wg - j.z + 1;
-  const auto record = [&](int i) { return ((long long)(2 * (j.z + i) + (i == 0 ? j.w : 0)) * kRows + row); };
-  float top = kNegFltMax;
-  for (int i = lane; i < n; i += 64) top = fmaxf(top, a.rec_ml[record(i) * 2]);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-  float l = 0.f;
-  for (int i = lane; i < n; i += 64)
-    l += a.rec_ml[record(i) * 2 + 1] * __builtin_amdgcn_exp2f(a.rec_ml[record(i) * 2] - top);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
-  float o[kPer];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave % PER_ROW;
+  const int group = j.y / a.row_blocks, block = j.y % a.row_blocks;
+  const int row = blockIdx.y * (16 / PER_ROW) + wave / PER_ROW;
+  int head, R;
+  row_of<NT>(a, group * (RW / a.sets), block, row, head, R);
+  const bool live = R < a.rows;  // what other rows join is not stored
+  const int n = j.w - (j.z >> 1) + 1;
+  float m = kNegFltMax, l = 0.f, o[kPer];
 #pragma unroll
   for (int e = 0; e < kPer; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int i = wave % PER_ROW; i < n; i += PER_ROW) {
-    const long long r = record(i);
-    const float f = __builtin_amdgcn_exp2f(a.rec_ml[r * 2] - top);
-    const float* from = a.rec_o + r * D + lane * kPer;
+  for (int i0 = sub; live && i0 < n; i0 += 4 * PER_ROW) {
+    float pm[4], pl[4], po[4][kPer];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) o[e] += f * from[e];
+    for (int u = 0; u < 4; ++u) {
+      const int i = min(i0 + u * PER_ROW, n - 1);
+      const long long r = (long long)(i == 0 ? j.z : 2 * ((j.z >> 1) + i)) * kRows + row;
+      pm[u] = a.rec_ml[2 * r];
+      pl[u] = a.rec_ml[2 * r + 1];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) po[u][e] = a.rec_o[r * D + lane * kPer + e];
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) top = fmaxf(top, pm[u]);
+    float f = __builtin_amdgcn_exp2f(m - top);
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] *= f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (i0 + u * PER_ROW >= n) continue;
+      f = __builtin_amdgcn_exp2f(pm[u] - top);
+      l += f * pl[u];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) o[e] += f * po[u][e];
+    }
+    m = top;
   }
   if constexpr (PER_ROW > 1) {
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) sh[wave][lane * kPer + e] = o[e];
-    __syncthreads();
-    if (wave != 0) return;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      o[e] = 0.f;
-#pragma unroll
-      for (int i = 0; i < PER_ROW; ++i) o[e] += sh[i][lane * kPer + e];
+    for (int e = 0; e < kPer; ++e) sh_o[wave][lane * kPer + e] = o[e];
+    if (lane == 0) {
+      sh_ml[wave][0] = m;
+      sh_ml[wave][1] = l;
     }
+    __syncthreads();
+    if (sub != 0) return;
+    float top = m;
+#pragma unroll
+    for (int i = 1; i < PER_ROW; ++i) top = fmaxf(top, sh_ml[wave + i][0]);
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) o[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER_ROW; ++i) {
+      const float f = __builtin_amdgcn_exp2f(sh_ml[wave + i][0] - top);
+      l += f * sh_ml[wave + i][1];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) o[e] += f * sh_o[wave + i][lane * kPer + e];
+    }
+    m = top;
   }
-  const int R = row0 + row, t = R / a.G, h = head * a.G + R - t * a.G;
+  if (!live) return;
+  const int t = position(a, R), h = head * a.G + R - t * a.G;
   const float inv = 1.f / l;
   uint16_t* to = reinterpret_cast<uint16_t*>(a.out) + j.x * a.out_s[0] + t * a.out_s[1] + h * a.out_s[2] + lane * kPer;
   if constexpr (kPer == 1) {
@@ -660,63 +776,95 @@ __global__ __launch_bounds__(kThreads) void gqa_join_kernel(const DecodeArgs a) 
     for (int e = 0; e < kPer; e += 2)
       *reinterpret_cast<uint32_t*>(to + e) = pack2_bf16_canon<kRTNE>(o[e] * inv, o[e + 1] * inv);
   }
-  if (a.lse && lane == 0) a.lse[((long long)j.x * a.q_len + t) * a.Hq + h] = kLn2 * (top + __builtin_amdgcn_logf(l));
+  if (a.lse && lane == 0) a.lse[((long long)j.x * a.q_len + t) * a.Hq + h] = kLn2 * (m + __builtin_amdgcn_logf(l));
 }
 
-// How a call is laid out: query rows of a task, tasks, workgroups, and whether they
-// share the tiles out evenly (with a join) or take a whole task each.
+// How a call is laid out.
 struct Plan {
-  int nt, row_blocks, grid, split;
+  int nt, rw, sets;          // 16-row tiles of a wave, row sets of a task, and of those one kv head's
+  int row_blocks, per;       // tasks of a kv head's rows, and of a request
+  int grid, split;           // workgroups; whether they share the tiles evenly or take a task each
   long long tasks;
 };
 constexpr int kCus = 256;
-// Up to this many tiles in the longest request a call runs a workgroup for each
+// Up to this many tokens in the longest request a call runs a workgroup for each
 // task, without the plan's reads and the second launch.
-constexpr int kShortTiles = 4;
+constexpr long long kShort = 512;
 
-inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int width, Plan* p) {
-  const long long rows = (long long)(Hq / Hkv) * q_len;
-  p->nt = rows <= 16 ? 1 : (rows <= 32 || D == 256) ? 2 : 4;
-  p->row_blocks = (int)((rows + 16 * p->nt - 1) / (16 * p->nt));
-  p->tasks = (long long)B * Hkv * p->row_blocks;
-  const long long tiles = ((long long)page * width + kTile - 1) / kTile;
-  const long long slots = kCus * (D * p->nt <= 128 ? 2 : 1);
-  p->split = tiles > kShortTiles;
-  const long long grid = p->split ? (p->tasks >= slots ? slots : (p->tasks * tiles < slots ? p->tasks * tiles : slots)) : p->tasks;
-  if (grid > INT_MAX) return false;
-  p->grid = (int)grid;
-  return true;
+// A K cache whose tokens hold their heads side by side (strides: as the launcher's).
+inline bool token_major(const long long* strides) { return strides[8] > strides[7]; }
+inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int width, bool by_token, Plan* p) {
+  const long long rows = (long long)(Hq / Hkv) * q_len, most = (long long)page * width;
+  p->nt = rows <= 16 || D == 256 ? 1 : 2;
+  const long long sets = (rows + 16 * p->nt - 1) / (16 * p->nt);
+  p->sets = sets == 1 ? 1 : sets == 2 ? 2 : 4;
+  p->rw = p->sets;
+  p->split = p->sets > 1 || most > kShort;
+  // Rows of neighbouring heads: four waves that read them together read whole lines
+  // and neighbouring ones.
+  if (p->split && by_token)
+    while (p->rw < 4 && 16 * p->nt * p->rw < 64 && Hkv % (p->rw / p->sets * 2) == 0) p->rw *= 2;
+  p->row_blocks = (int)((sets + p->sets - 1) / p->sets);
+  const long long per = (long long)(Hkv / (p->rw / p->sets)) * p->row_blocks;
+  if (per > 65535) return false;
+  p->per = (int)per;
+  p->tasks = B * per;
+    const long long tile = 32LL * (4 / p->rw), tiles = (most + tile - 1) / tile, slots = per_cu(D, p->nt) * kCus;
+  p->grid = (int)(p->tasks >= slots || p->tasks * tiles >= slots ? slots : p->tasks * tiles);
+  return p->tasks <= INT_MAX;
 }
-inline size_t record_bytes(const Plan& p, int D) { return (size_t)2 * p.grid * 16 * p.nt * (D + 2) * 4; }
+inline size_t record_bytes(const Plan& p, int D) { return (size_t)2 * p.grid * 16 * p.nt * p.rw * (D + 2) * 4; }
+// One entry for each task or run, whichever are fewer.
+inline long long join_count(const Plan& p) { return p.tasks < p.grid ? p.tasks : p.grid; }
 
-template <int D, bool FP8, int NT>
-int launch(DecodeArgs& a, const Plan& p, hipStream_t stream) {
-  hipLaunchKernelGGL((gqa_decode_kernel<D, FP8, NT>), dim3(p.grid), dim3(kThreads), 0, stream, a, p.split);
-  if (p.split) {
-    const int rows = a.rows < 16 * NT ? a.rows : 16 * NT;
-    if (p.tasks * 8 >= p.grid)
-      hipLaunchKernelGGL((gqa_join_kernel<D, NT, 1>), dim3(p.grid, (rows + 3) / 4), dim3(kThreads), 0, stream, a);
+template <int D, bool FP8, int NT, int RW, bool SHARED>
+int launch(const DecodeArgs& a, const Plan& p, hipStream_t stream) {
+  if (!p.split) {
+    if constexpr (RW == 1) {
+      using C = Shape<D, FP8, NT, 1, false, false>;
+      hipLaunchKernelGGL((gqa_decode_kernel<C>), dim3(a.B, p.per), dim3(C::kThreads), 0, stream, a);
+    }
+  } else {
+    using C = Shape<D, FP8, NT, RW, SHARED, true>;
+    hipLaunchKernelGGL((gqa_decode_kernel<C>), dim3(p.grid), dim3(C::kThreads), 0, stream, a);
+    // Records of a row: as many as runs share a task, or two ends of a run. A wave takes
+    // four at once.
+    const long long n = p.grid / p.tasks + 2, count = join_count(p);
+    const int rows = p.row_blocks > 1 || p.rw > p.sets ? C::kRows : a.rows;
+    if (n <= 4)
+      hipLaunchKernelGGL((gqa_join_kernel<D, NT, RW, 1>), dim3(count, (rows + 15) / 16), dim3(1024), 0, stream, a);
+    else if (n <= 16)
+      hipLaunchKernelGGL((gqa_join_kernel<D, NT, RW, 4>), dim3(count, (rows + 3) / 4), dim3(1024), 0, stream, a);
     else
-      hipLaunchKernelGGL((gqa_join_kernel<D, NT, 4>), dim3(p.grid, rows), dim3(kThreads), 0, stream, a);
+      hipLaunchKernelGGL((gqa_join_kernel<D, NT, RW, 16>), dim3(count, rows), dim3(1024), 0, stream, a);
   }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : (int)e;
 }
 
+// NT 1 of up to 128 dims is one row set.
+template <int D, bool FP8, int NT>
+int with_rw(const DecodeArgs& a, const Plan& p, hipStream_t st) {
+  if constexpr (NT > 1 || D == 256)
+    if (p.sets > 1) return p.rw == 2 ? launch<D, FP8, NT, 2, true>(a, p, st) : launch<D, FP8, NT, 4, true>(a, p, st);
+  return p.rw == 1   ? launch<D, FP8, NT, 1, false>(a, p, st)
+         : p.rw == 2 ? launch<D, FP8, NT, 2, false>(a, p, st)
+                     : launch<D, FP8, NT, 4, false>(a, p, st);
+}
 template <bool FP8>
-int dispatch(DecodeArgs& a, const Plan& p, int D, hipStream_t st) {
-  if (D == 64) return p.nt == 1 ? launch<64, FP8, 1>(a, p, st) : p.nt == 2 ? launch<64, FP8, 2>(a, p, st) : launch<64, FP8, 4>(a, p, st);
-  if (D == 128) return p.nt == 1 ? launch<128, FP8, 1>(a, p, st) : p.nt == 2 ? launch<128, FP8, 2>(a, p, st) : launch<128, FP8, 4>(a, p, st);
-  return p.nt == 1 ? launch<256, FP8, 1>(a, p, st) : launch<256, FP8, 2>(a, p, st);
+int dispatch(const DecodeArgs& a, const Plan& p, int D, hipStream_t st) {
+  if (D == 256) return with_rw<256, FP8, 1>(a, p, st);
+  if (D == 64) return p.nt == 1 ? with_rw<64, FP8, 1>(a, p, st) : with_rw<64, FP8, 2>(a, p, st);
+  return p.nt == 1 ? with_rw<128, FP8, 1>(a, p, st) : with_rw<128, FP8, 2>(a, p, st);
 }
 
 // -2 head_dim, -3 heads, -4 sizes, -5 page; 0 where the call can be planned.
 inline int check_sizes(int B, int q_len, int Hq, int Hkv, int D, int page, int width) {
   if (D != 64 && D != 128 && D != 256) return -2;
-  if (Hkv < 1 || Hq < Hkv || Hq % Hkv != 0) return -3;
+  if (Hkv < 1 || Hq < Hkv || Hq % Hkv != 0 || Hq > kMaxHeads) return -3;
   if (B < 0 || q_len < 1 || q_len > kMaxQLen) return -4;
   if (page < 16 || (page & (page - 1)) != 0) return -5;
-  if (width < 1) return -11;
+  if (width < 1 || (long long)page * width > kMaxTokens) return -11;
   return 0;
 }
 
@@ -725,12 +873,13 @@ inline int check_sizes(int B, int q_len, int Hq, int Hkv, int D, int page, int w
 
 extern "C" {
 
-size_t moonmath_gqa_decode_workspace(int B, int q_len, int Hq, int Hkv, int head_dim, int page, int max_blocks) {
+size_t moonmath_gqa_decode_workspace(int B, int q_len, int Hq, int Hkv, int head_dim, int page, int max_blocks,
+                                     const long long* strides) {
   using namespace mm::gqa;
   Plan p;
-  if (B == 0 || check_sizes(B, q_len, Hq, Hkv, head_dim, page, max_blocks) != 0) return 0;
-  if (!plan_call(B, q_len, Hq, Hkv, head_dim, page, max_blocks, &p) || !p.split) return 0;
-  return record_bytes(p, head_dim) + (size_t)p.grid * sizeof(int4);
+  if (B == 0 || !strides || check_sizes(B, q_len, Hq, Hkv, head_dim, page, max_blocks) != 0) return 0;
+  if (!plan_call(B, q_len, Hq, Hkv, head_dim, page, max_blocks, token_major(strides), &p) || !p.split) return 0;
+  return record_bytes(p, head_dim) + (size_t)join_count(p) * sizeof(int4);
 }
 
 int launch_gqa_decode_paged(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
@@ -743,13 +892,16 @@ int launch_gqa_decode_paged(const void* q, const void* k_cache, const void* v_ca
   if (num_blocks < 1) return -11;
   if (B == 0) return 0;
   if (!q || !k_cache || !v_cache || !out || !seq_lens || !block_table || !strides || !k_scale != !v_scale) return -6;
-  Plan p;
-  if (!plan_call(B, q_len, Hq, Hkv, head_dim, page, max_blocks, &p)) return -8;
-  if (p.split && !workspace) return -6;
   DecodeArgs a{};
-  a.q = (const char*)q;
   a.k = make_cache(k_cache, k_scale, strides + 6);
   a.v = make_cache(v_cache, v_scale, strides + 11);
+  // A lane adds up to 15 rows to a page's address in 32 bits.
+  const long long widest = 1LL << 26;
+  if (a.k.row_s < 0 || a.v.row_s < 0 || a.k.row_s > widest || a.v.row_s > widest) return -9;
+  Plan p;
+  if (!plan_call(B, q_len, Hq, Hkv, head_dim, page, max_blocks, token_major(strides), &p)) return -8;
+  if (p.split && !workspace) return -6;
+  a.q = (const char*)q;
   a.out = (char*)out;
   a.lse = (float*)lse;
   a.seq_lens = (const int*)seq_lens;
@@ -759,23 +911,23 @@ int launch_gqa_decode_paged(const void* q, const void* k_cache, const void* v_ca
     a.out_s[i] = strides[3 + i];
   }
   a.table_s = strides[16];
-  // A lane adds up to 15 rows to a page's address in 32 bits.
-  const long long widest = 1LL << 26;
-  if (a.k.row_s < 0 || a.v.row_s < 0 || a.k.row_s > widest || a.v.row_s > widest) return -9;
   a.rec_o = (float*)workspace;
-  a.rec_ml = a.rec_o + (size_t)2 * p.grid * 16 * p.nt * head_dim;
-  a.joins = (int4*)(a.rec_ml + (size_t)2 * p.grid * 16 * p.nt * 2);
+  a.rec_ml = a.rec_o + (size_t)2 * p.grid * 16 * p.nt * p.rw * head_dim;
+  a.joins = (int4*)(a.rec_ml + (size_t)2 * p.grid * 16 * p.nt * p.rw * 2);
   a.B = B;
   a.q_len = q_len;
   a.Hq = Hq;
-  a.Hkv = Hkv;
   a.G = Hq / Hkv;
   a.rows = a.G * q_len;
+  a.sets = p.sets;
   a.row_blocks = p.row_blocks;
+  a.per = p.per;
+  a.joins_by_task = p.tasks <= p.grid;
   a.num_blocks = num_blocks;
   a.width = max_blocks;
   a.page_shift = __builtin_ctz(page);
   a.scale2 = scale * kLog2e;
+  a.inv_g = 1.f / (float)a.G;
   return k_scale ? dispatch<true>(a, p, head_dim, (hipStream_t)stream) : dispatch<false>(a, p, head_dim, (hipStream_t)stream);
 }
 

@@ -30,6 +30,8 @@ __all__ = ["gqa_decode_paged", "gqa_kv_read", "gqa_kv_write"]
 _FP8 = torch.float8_e4m3fn
 _DIMS = (64, 128, 256)
 _MAX_Q_LEN = 8
+_MAX_HEADS = 1 << 16
+_MAX_TOKENS = (1 << 31) - 64
 _MAX_ROW_STRIDE = 1 << 26
 
 
@@ -205,14 +207,16 @@ def gqa_decode_paged(q, k_cache, v_cache, seq_lens, block_table, *, scale=None, 
     B, q_len, Hq = q4.shape[:3]
     if not 1 <= q_len <= _MAX_Q_LEN:
         raise ValueError(f"{who}: q_len must be in [1,{_MAX_Q_LEN}]")
-    if Hq < 1 or Hq % heads:
-        raise ValueError(f"{who}: Hq = {Hq} must be a multiple of the cache's {heads} heads")
+    if Hq < 1 or Hq % heads or Hq > _MAX_HEADS:
+        raise ValueError(f"{who}: Hq = {Hq} must be a multiple of the cache's {heads} heads, and at most 65536")
     _check_ints(seq_lens, "seq_lens", who)
     _check_ints(block_table, "block_table", who)
     if seq_lens.dim() != 1 or seq_lens.shape[0] != B or not seq_lens.is_contiguous():
         raise ValueError(f"{who}: seq_lens must be contiguous [B] = [{B}], got {list(seq_lens.shape)}")
     if block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] < 1:
         raise ValueError(f"{who}: block_table must be [B, max_blocks] with B = {B}, got {list(block_table.shape)}")
+    if block_table.shape[1] * page > _MAX_TOKENS:
+        raise ValueError(f"{who}: a request's table must hold at most 2^31 - 64 tokens")
     if block_table.shape[1] > 1 and block_table.stride(1) != 1:
         raise ValueError(f"{who}: block_table's last dim must be contiguous")
     if out is not None:
@@ -237,7 +241,7 @@ def gqa_decode_paged(q, k_cache, v_cache, seq_lens, block_table, *, scale=None, 
                        *_cache_strides(v_cache, v_scale), block_table.stride(0))
     p = _lib.ptr
     with torch.cuda.device(dev):
-        nbytes = _lib.lib.moonmath_gqa_decode_workspace(B, q_len, Hq, heads, D, page, width)
+        nbytes = _lib.lib.moonmath_gqa_decode_workspace(B, q_len, Hq, heads, D, page, width, strides)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         _run("launch_gqa_decode_paged", p(q), p(k_cache), p(v_cache), p(k_scale), p(v_scale), p(out), p(lse),
              p(seq_lens), p(block_table), B, q_len, Hq, heads, D, nb, page, width, strides, scale, p(ws),

@@ -276,7 +276,8 @@ int moonmath_pack_bf16(const void* in, void* out, int n, int round_mode, void* s
  * block's rows contiguous): 5 strides each, {block, head, row, scale block,
  * scale head}. page: rows of a block, a power of two, at least 16.
  * Codes: -2 head_dim, -3 heads, -4 sizes, -5 page or pairs, -6 null pointer,
- * -8 grid overflow, -9 row stride above 2^26, -11 bad block-table or pool geometry.
+ * -8 grid overflow, -9 row stride above 2^26, -11 bad block-table or pool geometry
+ * (a request's table holds at most 2^31 - 64 tokens).
  * ------------------------------------------------------------------------- */
 
 /* Rows of new tokens into their slots (block * page + row; int32, outside
@@ -301,7 +302,7 @@ int launch_gqa_kv_read(const void* k_cache, const void* v_cache, const void* k_s
  * page]); query head h reads kv head h / (Hq / Hkv). q, out: bf16 [B, q_len, Hq,
  * head_dim] (out may be q); lse: fp32 [B, q_len, Hq] contiguous or NULL, ln of the
  * softmax's sum. A query that sees no token: zeros, -inf. workspace:
- * moonmath_gqa_decode_workspace bytes (NULL where that is 0), 16-byte aligned, its
+ * moonmath_gqa_decode_workspace bytes for the same arguments (NULL where that is 0), 16-byte aligned, its
  * contents neither read nor kept across calls; calls that overlap need one each.
  * strides: q {batch, query, head}, out {batch, query, head}, k cache, v cache,
  * {block_table row}: 17. */
@@ -309,7 +310,8 @@ int launch_gqa_decode_paged(const void* q, const void* k_cache, const void* v_ca
                             const void* v_scale, void* out, void* lse, const void* seq_lens, const void* block_table,
                             int B, int q_len, int Hq, int Hkv, int head_dim, int num_blocks, int page, int max_blocks,
                             const long long* strides, float scale, void* workspace, void* stream);
-size_t moonmath_gqa_decode_workspace(int B, int q_len, int Hq, int Hkv, int head_dim, int page, int max_blocks);
+size_t moonmath_gqa_decode_workspace(int B, int q_len, int Hq, int Hkv, int head_dim, int page, int max_blocks,
+                                     const long long* strides);
 
 /* Rotary positions: pair p of each head of q [B, S, Hq, head_dim] and k [B, S,
  * Hk, head_dim] (Hk 0: q alone) turns by positions[axes[p]][b][s] * turns[p] of a

@@ -103,6 +103,8 @@ def test_refused_distance_of_tokens():
     ({"block_table": z(2, 2, dtype=I32)}, ValueError, "block_table must be \\[B, max_blocks\\]"),
     ({"block_table": z(3, 0, dtype=I32)}, ValueError, "block_table must be \\[B, max_blocks\\]"),
     ({"block_table": z(2, 3, dtype=I32).t()}, ValueError, "last dim must be contiguous"),
+    ({"block_table": z(3, 1, dtype=I32).expand(3, 1 << 27)}, ValueError, "at most 2\\^31 - 64 tokens"),
+    ({"q": z(1, 1, 64).expand(3, 65538, 64)}, ValueError, "at most 65536"),
     ({"scale": "x"}, ValueError, "could not convert"),
     ({"out": z(3, 4, 64, dtype=torch.float32)}, ValueError, "out must be bfloat16"),
     ({"out": z(3, 1, 4, 64)}, ValueError, "out must have q's shape"),
@@ -270,6 +272,7 @@ def test_launcher_codes():
         lib.launch_gqa_decode_paged(x, p, p, ks, vs, p, n, p, p, B, T, Hq, Hkv, D, nb, page, w, s, 1.0, ws, n))
     assert dec(D=80) == -2 and dec(Hkv=0) == -3 and dec(Hq=5) == -3 and dec(Hq=1) == -3
     assert dec(B=-1) == -4 and dec(T=0) == -4 and dec(T=9) == -4 and dec(page=8) == -5 and dec(page=24) == -5
+    assert dec(Hq=1 << 17) == -3 and dec(w=1 << 27) == -11
     assert dec(w=0) == -11 and dec(nb=0) == -11 and dec(x=n) == -6 and dec(ks=p) == -6 and dec(vs=p) == -6
     assert dec(s=None) == -6 and dec(w=1000) == -6  # a split without a workspace
     far = (ctypes.c_longlong * 17)()
@@ -292,10 +295,12 @@ def test_launcher_codes():
 def test_workspace():
     """Records depend on the call's shape and not on its lengths; short contexts, empty
     batches and sizes that are refused need none."""
-    ws = _lib.lib.moonmath_gqa_decode_workspace
-    assert ws(64, 1, 32, 8, 128, 64, 2) == 0 and ws(0, 1, 32, 8, 128, 64, 128) == 0 and ws(1, 1, 32, 8, 96, 64, 128) == 0
-    sizes = [ws(B, 1, 32, 8, 128, 64, 128) for B in (1, 4, 64, 1024)]
-    assert 0 < sizes[0] <= sizes[1] <= sizes[2] == sizes[3] < 64 << 20
+    heads, tokens = ((ctypes.c_longlong * 17)(*[0] * 6, *x) for x in ((1 << 20, 1 << 13, 128), (1 << 16, 128, 1024)))
+    ws = lambda B, D=128, w=128, s=heads: _lib.lib.moonmath_gqa_decode_workspace(B, 1, 32, 8, D, 64, w, s)  # noqa: E731
+    assert ws(64, w=2) == 0 and ws(0) == 0 and ws(1, D=96) == 0 and ws(1, s=None) == 0
+    for s in (heads, tokens):
+        sizes = [ws(B, s=s) for B in (1, 4, 64, 1024)]
+        assert 0 < sizes[0] <= sizes[1] <= sizes[2] <= sizes[3] <= sizes[2] + (16 << 10) < 64 << 20
 
 
 def test_native_path_leaves_cpu_calls():
