@@ -401,7 +401,7 @@ struct Run {
   long long total;
   long long start, end;   // tiles of all tasks, in order
   long long before;       // tiles before request b
-  int runs, b;
+  int runs, b, len;       // and that request's length
 };
 // Every thread calls it. Requests are taken THREADS at a time, one for each thread, and
 // a prefix sum finds the one that holds the run's first tile.
@@ -409,12 +409,13 @@ template <int THREADS, int TILE>
 __device__ Run find_run(const DecodeArgs& a, int wg, int grid) {
   constexpr int kWaves = THREADS / 64;
   __shared__ int sh_sum[2][kWaves];
-  __shared__ long long sh_found[2];
+  __shared__ long long sh_found[3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // A wave's 64 requests have fewer than 2^32 tiles; sums over waves are 64 bits.
   static_assert(TILE >= 32, "64 requests of at most kMaxTokens");
-  const auto group = [&](int b0, int turn, int& n, int& incl, long long& ahead, long long& sum) {
-    n = b0 + tid < a.B ? tiles_of<TILE>(clamped(a, a.seq_lens[b0 + tid])) : 0;
+  const auto group = [&](int b0, int turn, int& len, int& n, int& incl, long long& ahead, long long& sum) {
+    len = b0 + tid < a.B ? clamped(a, a.seq_lens[b0 + tid]) : 0;
+    n = tiles_of<TILE>(len);
     incl = wave_incl_scan(n);
     if (lane == 63) sh_sum[turn][wave] = incl;
     __syncthreads();
@@ -425,10 +426,10 @@ __device__ Run find_run(const DecodeArgs& a, int wg, int grid) {
       sum += (uint32_t)sh_sum[turn][i];
     }
   };
-  int n, incl;
+  int len, n, incl;
   long long ahead, sum, total = 0;
   for (int b0 = 0, turn = 0; b0 < a.B; b0 += THREADS, turn ^= 1) {
-    group(b0, turn, n, incl, ahead, sum);
+    group(b0, turn, len, n, incl, ahead, sum);
     total += sum;
   }
   Run run{};
@@ -442,12 +443,13 @@ __device__ Run find_run(const DecodeArgs& a, int wg, int grid) {
   for (int b0 = 0, turn = 0; b0 < a.B; b0 += THREADS, turn ^= 1) {
     if (a.B > THREADS) {
       __syncthreads();
-      group(b0, turn, n, incl, ahead, sum);
+      group(b0, turn, len, n, incl, ahead, sum);
     }
     const long long before = (base + ahead + (uint32_t)incl - (uint32_t)n) * a.per;
     if (run.start >= before && run.start < before + (long long)n * a.per) {
       sh_found[0] = b0 + tid;
       sh_found[1] = before;
+      sh_found[2] = len;
     }
     base += sum;
     if (run.start < base * a.per) break;
@@ -455,6 +457,7 @@ __device__ Run find_run(const DecodeArgs& a, int wg, int grid) {
   __syncthreads();
   run.b = uniform((int)sh_found[0]);
   run.before = uniform(sh_found[1]);
+  run.len = uniform((int)sh_found[2]);
   return run;
 }
 
@@ -468,6 +471,55 @@ __device__ __forceinline__ void row_of(const DecodeArgs& a, int head0, int block
 // r / G for r below q_len * G: exact, as (r + 1/2) / G lies 1 / (2 G) from a whole number.
 __device__ __forceinline__ int position(const DecodeArgs& a, int r) { return (int)(((float)r + 0.5f) * a.inv_g); }
 
+// The part of a task that a workgroup takes, all of it wave-uniform.
+struct Segment {
+  long long before;           // tiles before request b
+  int b, task, len, tiles;    // the request's length and a task's tiles
+  int tile0, tile1;
+  int head0, block;           // the task's first kv head and block of its rows
+};
+template <class C>
+__device__ __forceinline__ void place(const DecodeArgs& a, Segment& x) {
+  const int group = a.row_blocks == 1 ? x.task : x.task / a.row_blocks;
+  x.block = a.row_blocks == 1 ? 0 : x.task - group * a.row_blocks;
+  x.head0 = a.sets == C::RW ? group : a.sets * 2 == C::RW ? group * 2 : group * 4;
+}
+
+// A wave's first loads for a segment: its query rows and its first step.
+template <class C>
+__device__ __forceinline__ void begin(const DecodeArgs& a, const Segment& x, Rows<C>& w, Step<C>& s, int rw, int tg,
+                                      int lane) {
+  constexpr int NT = C::NT;
+  const int st = x.tile0 * C::kGroups + tg, n = lane & 15, g = lane >> 4;
+  const ConstInts table = (ConstInts)(uintptr_t)(a.table + (long long)x.b * a.table_s);
+  const Pages<C> pg = step_pages<C>(a, table, st * C::kStep);
+  int head, row0;
+  row_of<NT>(a, x.head0, x.block, rw * 16 * NT, head, row0);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = row0 + 16 * nt + n;
+    const bool live = r < a.rows;
+    const int t = live ? position(a, r) : a.q_len - 1;
+    w.pos[nt] = t;
+    const char* qr = a.q + 2 * (x.b * a.q_s[0] + t * a.q_s[1] + (head * a.G + (live ? r - t * a.G : 0)) * a.q_s[2]);
+#pragma unroll
+    for (int c = 0; c < C::D / 32; ++c) {
+      // dims of MFMA c for lane group g, as K's loads have them
+      const int d = C::FP8 ? 64 * (c / 2) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g;
+      u32x4 y = *reinterpret_cast<const u32x4*>(qr + 2 * d);
+      if (!live) y = u32x4{0u, 0u, 0u, 0u};
+      w.q[nt][c] = __builtin_bit_cast(bf16x8, y);
+    }
+  }
+  // K before V here as in the loop: the compiler's wait for K there counts the loads
+  // that may have been issued since on every way into it.
+  sched_fence();
+  load_k<C>(a, s, pg, st * C::kStep, head, lane);
+  sched_fence();
+  load_v<C>(a, s, pg, st * C::kStep, head, lane);
+  sched_fence();
+}
+
 // SPLIT: the workgroup takes its run of all tasks' tiles. Otherwise a whole task:
 // nothing is planned, and the first step is loaded before the request's length is there.
 template <class C>
@@ -478,112 +530,87 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
   __shared__ float sh_o[kWaves][16][kPitch];
   __shared__ float sh_ml[C::kGroups][C::kRows][2];
 
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int wave = uniform(tid >> 6), rw = wave % C::RW, tg = wave / C::RW;
 
-  int wg = 0, b, task = 0, grid = 0;
+  int wg = 0, grid = 0;
   Run run{};
+  Segment x{};
+  bool more = true;
   if constexpr (SPLIT) {
     grid = gridDim.x;
     wg = xcd_remap(blockIdx.x, grid);
     run = find_run<kThreads, C::kTile>(a, wg, grid);
     if (!a.joins_by_task && tid == 0) a.joins[wg] = int4{-1, 0, 0, 0};
-    b = run.b;
-  } else {
-    b = blockIdx.x;
-    task = blockIdx.y;
-    run.end = 1;
-  }
-  bool first = true;
-  long long at = run.start, before = run.before;
-  while (at < run.end && b < a.B) {
-    int len = 0, tiles = 0, tile0 = 0, tile1 = 0;
-    if constexpr (SPLIT) {
-      len = len_of(a, b);
-      tiles = tiles_of<C::kTile>(len);
-      if (at - before >= (long long)tiles * a.per) {  // done with request b
-        before += (long long)tiles * a.per;
-        ++b;
-        continue;
-      }
-      task = uniform((int)((at - before) / tiles));
-      tile0 = uniform((int)((at - before) - (long long)task * tiles));
-      tile1 = uniform((int)min((long long)tiles, tile0 + (run.end - at)));
+    more = run.start < run.end;
+    if (more) {
+      x.b = run.b;
+      x.before = run.before;
+      x.len = run.len;
+      x.tiles = tiles_of<C::kTile>(x.len);
+      x.task = uniform((int)((run.start - x.before) / x.tiles));
+      x.tile0 = uniform((int)(run.start - x.before - (long long)x.task * x.tiles));
+      x.tile1 = uniform((int)min((long long)x.tiles, x.tile0 + (run.end - run.start)));
     }
-    const int group = a.row_blocks == 1 ? task : task / a.row_blocks;
-    const int block = a.row_blocks == 1 ? 0 : task - group * a.row_blocks;
-    const int head0 = a.sets == C::RW ? group : a.sets * 2 == C::RW ? group * 2 : group * 4;
-    const ConstInts table = (ConstInts)(uintptr_t)(a.table + (long long)b * a.table_s);
-
-    // This wave's first step, and its query rows.
-    int st = tile0 * C::kGroups + tg;
-    Step<C> s;
-    Pages<C> pg = step_pages<C>(a, table, st * C::kStep);
+  } else {
+    x.b = blockIdx.x;
+    x.task = blockIdx.y;
+  }
+  long long at = run.start;
+  bool first = true;
+  while (more) {
+    place<C>(a, x);
     Rows<C> w;
-    const int n = lane & 15, g = lane >> 4;
-    int head, row0;
-    row_of<NT>(a, head0, block, rw * 16 * NT, head, row0);
+    Step<C> s;
+    begin<C>(a, x, w, s, rw, tg, lane);
+    if constexpr (!SPLIT) {
+      x.len = len_of(a, x.b);
+      x.tile1 = x.tiles = tiles_of<C::kTile>(x.len);
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = row0 + 16 * nt + n;
-      const bool live = r < a.rows;
-      const int t = live ? position(a, r) : a.q_len - 1;
-      w.pos[nt] = t;
       w.m[nt] = kNegFltMax;
       w.l[nt] = 0.f;
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) w.o[nt][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const char* qr = a.q + 2 * (b * a.q_s[0] + t * a.q_s[1] + (head * a.G + (live ? r - t * a.G : 0)) * a.q_s[2]);
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        // dims of MFMA c for lane group g, as K's loads have them
-        const int d = C::FP8 ? 64 * (c / 2) + 16 * g + 8 * (c & 1) : 32 * c + 8 * g;
-        u32x4 x = *reinterpret_cast<const u32x4*>(qr + 2 * d);
-        if (!live) x = u32x4{0u, 0u, 0u, 0u};
-        w.q[nt][c] = __builtin_bit_cast(bf16x8, x);
-      }
-    }
-    // K before V here as in the loop: the compiler's wait for K there counts the loads
-    // that may have been issued since on every way into it.
-    sched_fence();
-    load_k<C>(a, s, pg, st * C::kStep, head, lane);
-    sched_fence();
-    load_v<C>(a, s, pg, st * C::kStep, head, lane);
-    if constexpr (!SPLIT) {
-      len = len_of(a, b);
-      tile1 = tiles = tiles_of<C::kTile>(len);
     }
 
-    // Its steps are every kGroups-th one. Those from s_full on hold tokens that some
-    // position does not see: a step's worth and q_len - 1, in two steps at most. Loads
-    // past the last step repeat it: one under a branch would make the compiler wait
-    // for all of them.
-    const int s_end = min(tile1 * C::kGroups, tiles_of<C::kStep>(len));
-    if (st < s_end && row0 < a.rows) {
-      const int s_last = st + (s_end - 1 - st) / C::kGroups * C::kGroups;
-      const int seen = len - a.q_len + 1;
-      const int s_full = seen > 0 ? seen / C::kStep : 0;
-      int next = min(st + C::kGroups, s_last);
-      pg = step_pages<C>(a, table, next * C::kStep);
-      for (; st <= s_last && st < s_full; st += C::kGroups) {
-        const int after = min(next + C::kGroups, s_last);
-        const Pages<C> pa = step_pages<C>(a, table, after * C::kStep);
-        compute_step<C, false>(a, w, s, st * C::kStep, len, pg, next * C::kStep, head, lane);
-        pg = pa;
-        next = after;
-      }
-      while (st <= s_last) {
-        compute_step<C, true>(a, w, s, st * C::kStep, len, pg, 0, head, lane);
-        st += C::kGroups;
-        if (C::kGroups > 1 || st > s_last) break;  // a wave of several has one such step
-        pg = step_pages<C>(a, table, st * C::kStep);
-        load_k<C>(a, s, pg, st * C::kStep, head, lane);
-        load_v<C>(a, s, pg, st * C::kStep, head, lane);
+    // A wave's steps are every kGroups-th one. Those from s_full on hold tokens that
+    // some position does not see: a step's worth and q_len - 1, in two steps at most.
+    // Loads past the last step repeat it: one under a branch would make the compiler
+    // wait for all of them.
+    {
+      const ConstInts table = (ConstInts)(uintptr_t)(a.table + (long long)x.b * a.table_s);
+      int head, row0;
+      row_of<NT>(a, x.head0, x.block, rw * 16 * NT, head, row0);
+      int st = x.tile0 * C::kGroups + tg;
+      const int s_end = min(x.tile1 * C::kGroups, tiles_of<C::kStep>(x.len));
+      if (st < s_end && row0 < a.rows) {
+        const int s_last = st + (s_end - 1 - st) / C::kGroups * C::kGroups;
+        const int seen = x.len - a.q_len + 1;
+        const int s_full = seen > 0 ? seen / C::kStep : 0;
+        int next = min(st + C::kGroups, s_last);
+        Pages<C> pg = step_pages<C>(a, table, next * C::kStep);
+        for (; st <= s_last && st < s_full; st += C::kGroups) {
+          const int after = min(next + C::kGroups, s_last);
+          const Pages<C> pa = step_pages<C>(a, table, after * C::kStep);
+          compute_step<C, false>(a, w, s, st * C::kStep, x.len, pg, next * C::kStep, head, lane);
+          pg = pa;
+          next = after;
+        }
+        while (st <= s_last) {
+          compute_step<C, true>(a, w, s, st * C::kStep, x.len, pg, 0, head, lane);
+          st += C::kGroups;
+          if (C::kGroups > 1 || st > s_last) break;  // a wave of several has one such step
+          pg = step_pages<C>(a, table, st * C::kStep);
+          load_k<C>(a, s, pg, st * C::kStep, head, lane);
+          load_v<C>(a, s, pg, st * C::kStep, head, lane);
+        }
       }
     }
 
-    // Join the waves.
-    const bool whole = !SPLIT || (tile0 == 0 && tile1 == tiles);
+    // Join the waves. The barriers wait for LDS alone.
+    const bool whole = !SPLIT || (x.tile0 == 0 && x.tile1 == x.tiles);
     const int rec = 2 * wg + (first ? 0 : 1);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -593,7 +620,7 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
         sh_ml[tg][(rw * NT + nt) * 16 + n][1] = w.l[nt];
       }
     }
-    __syncthreads();
+    lds_reads_done_barrier();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       {
@@ -611,14 +638,14 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
             *reinterpret_cast<f32x4*>(to + (D / 16) * r + j) =
                 f32x4{w.o[nt][j][r] * f, w.o[nt][j + 1][r] * f, w.o[nt][j + 2][r] * f, w.o[nt][j + 3][r] * f};
       }
-      __syncthreads();
+      lds_reads_done_barrier();
       {
         // The row sets' tiles nt: kAcross threads for each of 16 * RW rows, kPer dims each.
         constexpr int kAcross = kThreads / (16 * C::RW), kPer = D / kAcross;
         const int set = tid / (16 * kAcross), in = tid / kAcross % 16, d0 = tid % kAcross * kPer;
         const int row = (set * NT + nt) * 16 + in;
         int h, R;
-        row_of<NT>(a, head0, block, row, h, R);
+        row_of<NT>(a, x.head0, x.block, row, h, R);
         if (R < a.rows) {
           float top = sh_ml[0][row][0];
 #pragma unroll
@@ -635,15 +662,15 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
           }
           if (whole) {
             const int t = position(a, R), hq = h * a.G + R - t * a.G;
-            const bool none = len - a.q_len + t + 1 <= 0;  // the row sees no token
+            const bool none = x.len - a.q_len + t + 1 <= 0;  // the row sees no token
             const float inv = 1.f / l;
-            char* to = a.out + 2 * (b * a.out_s[0] + t * a.out_s[1] + hq * a.out_s[2] + d0);
+            char* to = a.out + 2 * (x.b * a.out_s[0] + t * a.out_s[1] + hq * a.out_s[2] + d0);
 #pragma unroll
             for (int j = 0; j < kPer; j += 2)
               *reinterpret_cast<uint32_t*>(to + 2 * j) =
                   none ? 0u : pack2_bf16_canon<kRTNE>(o[j] * inv, o[j + 1] * inv);
             if (a.lse && d0 == 0)
-              a.lse[((long long)b * a.q_len + t) * a.Hq + hq] =
+              a.lse[((long long)x.b * a.q_len + t) * a.Hq + hq] =
                   none ? -__builtin_inff() : kLn2 * (top + __builtin_amdgcn_logf(l));
           } else {
             float* to = a.rec_o + ((long long)rec * C::kRows + row) * D + d0;
@@ -656,27 +683,42 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
           }
         }
       }
-      __syncthreads();
+      lds_reads_done_barrier();
     }
     if constexpr (!SPLIT) return;
-    if (tile1 == tiles && tid == 0) {
+    if (x.tile1 == x.tiles && tid == 0) {
       // The task ends in this run. Where it began in an earlier one: that run, and which
       // of its two records holds the beginning (its first segment's, or its last's).
       int4 join{-1, 0, 0, 0};
       if (!whole) {
-        const long long began = before + (long long)task * tiles;
+        const long long began = x.before + (long long)x.task * x.tiles;
         int w0 = (int)(began * run.runs / run.total);
         while (run_start(run.total, run.runs, w0) > began) --w0;
         while (run_start(run.total, run.runs, w0 + 1) <= began) ++w0;
-        join = int4{b, task, 2 * w0 + (run_start(run.total, run.runs, w0) == began ? 0 : 1), wg};
+        join = int4{x.b, x.task, 2 * w0 + (run_start(run.total, run.runs, w0) == began ? 0 : 1), wg};
       }
       if (a.joins_by_task)
-        a.joins[b * a.per + task] = join;
+        a.joins[x.b * a.per + x.task] = join;
       else if (!whole)
         a.joins[wg] = join;  // of the first segment only: one for each run
     }
     first = false;
-    at += tile1 - tile0;
+    at += x.tile1 - x.tile0;
+    more = at < run.end;
+    x.tile0 = 0;
+    if (more && ++x.task == a.per) {
+      x.task = 0;
+      do {
+        x.before += (long long)x.tiles * a.per;
+        if (++x.b >= a.B) {
+          more = false;
+          break;
+        }
+        x.len = len_of(a, x.b);
+        x.tiles = tiles_of<C::kTile>(x.len);
+      } while (x.tiles == 0);
+    }
+    x.tile1 = (int)min((long long)x.tiles, run.end - at);
   }
 
   // Requests without a token: zeros.
@@ -694,88 +736,80 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
 }
 
 // Joins the records of a task that several runs hold: rows of O and (m, l), in an order
-// that the call's shape and lengths alone decide. PER_ROW of a workgroup's 16 waves
-// share a row's records, each with a running maximum over its own, four loaded at once.
+// that the call's shape and lengths alone decide. D / 4 lanes hold a row (16 bytes
+// each); PER_ROW such groups share a row's records, each with a running maximum over
+// its own, four loaded at once.
+constexpr int kJoinThreads = 512;
 template <int D, int NT, int RW, int PER_ROW>
-__global__ __launch_bounds__(1024) void gqa_join_kernel(const DecodeArgs a) {
-  constexpr int kRows = 16 * NT * RW, kPer = D / 64;
-  __shared__ float sh_o[PER_ROW > 1 ? 16 : 1][D];
-  __shared__ float sh_ml[16][2];
+__global__ __launch_bounds__(kJoinThreads) void gqa_join_kernel(const DecodeArgs a) {
+  constexpr int kRows = 16 * NT * RW, kLanes = D / 4, kGroups = kJoinThreads / kLanes;
+  __shared__ f32x4 sh_o[PER_ROW > 1 ? kGroups : 1][kLanes];
+  __shared__ float sh_ml[kGroups][2];
   const int4 j = a.joins[blockIdx.x];
   if (j.x < 0) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = wave % PER_ROW;
+  const int lane = threadIdx.x % kLanes, mine = threadIdx.x / kLanes, sub = mine % PER_ROW;
   const int group = j.y / a.row_blocks, block = j.y % a.row_blocks;
-  const int row = blockIdx.y * (16 / PER_ROW) + wave / PER_ROW;
+  const int row = blockIdx.y * (kGroups / PER_ROW) + mine / PER_ROW;
   int head, R;
   row_of<NT>(a, group * (RW / a.sets), block, row, head, R);
-  const bool live = R < a.rows;  // what other rows join is not stored
+  const bool live = row < kRows && R < a.rows;  // what other rows join is not stored
   const int n = j.w - (j.z >> 1) + 1;
-  float m = kNegFltMax, l = 0.f, o[kPer];
-#pragma unroll
-  for (int e = 0; e < kPer; ++e) o[e] = 0.f;
+  float m = kNegFltMax, l = 0.f;
+  f32x4 o{0.f, 0.f, 0.f, 0.f};
   for (int i0 = sub; live && i0 < n; i0 += 4 * PER_ROW) {
-    float pm[4], pl[4], po[4][kPer];
+    float pm[4], pl[4];
+    f32x4 po[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int i = min(i0 + u * PER_ROW, n - 1);
       const long long r = (long long)(i == 0 ? j.z : 2 * ((j.z >> 1) + i)) * kRows + row;
       pm[u] = a.rec_ml[2 * r];
       pl[u] = a.rec_ml[2 * r + 1];
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) po[u][e] = a.rec_o[r * D + lane * kPer + e];
+      po[u] = *reinterpret_cast<const f32x4*>(a.rec_o + r * D + lane * 4);
     }
     float top = m;
 #pragma unroll
     for (int u = 0; u < 4; ++u) top = fmaxf(top, pm[u]);
     float f = __builtin_amdgcn_exp2f(m - top);
     l *= f;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) o[e] *= f;
+    o *= f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       if (i0 + u * PER_ROW >= n) continue;
       f = __builtin_amdgcn_exp2f(pm[u] - top);
       l += f * pl[u];
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) o[e] += f * po[u][e];
+      o += f * po[u];
     }
     m = top;
   }
   if constexpr (PER_ROW > 1) {
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) sh_o[wave][lane * kPer + e] = o[e];
+    sh_o[mine][lane] = o;
     if (lane == 0) {
-      sh_ml[wave][0] = m;
-      sh_ml[wave][1] = l;
+      sh_ml[mine][0] = m;
+      sh_ml[mine][1] = l;
     }
     __syncthreads();
     if (sub != 0) return;
     float top = m;
 #pragma unroll
-    for (int i = 1; i < PER_ROW; ++i) top = fmaxf(top, sh_ml[wave + i][0]);
+    for (int i = 1; i < PER_ROW; ++i) top = fmaxf(top, sh_ml[mine + i][0]);
     l = 0.f;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) o[e] = 0.f;
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < PER_ROW; ++i) {
-      const float f = __builtin_amdgcn_exp2f(sh_ml[wave + i][0] - top);
-      l += f * sh_ml[wave + i][1];
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) o[e] += f * sh_o[wave + i][lane * kPer + e];
+      const float f = __builtin_amdgcn_exp2f(sh_ml[mine + i][0] - top);
+      l += f * sh_ml[mine + i][1];
+      o += f * sh_o[mine + i][lane];
     }
     m = top;
   }
   if (!live) return;
   const int t = position(a, R), h = head * a.G + R - t * a.G;
-  const float inv = 1.f / l;
-  uint16_t* to = reinterpret_cast<uint16_t*>(a.out) + j.x * a.out_s[0] + t * a.out_s[1] + h * a.out_s[2] + lane * kPer;
-  if constexpr (kPer == 1) {
-    *to = (uint16_t)pack2_bf16_canon<kRTNE>(o[0] * inv, 0.f);
-  } else {
-#pragma unroll
-    for (int e = 0; e < kPer; e += 2)
-      *reinterpret_cast<uint32_t*>(to + e) = pack2_bf16_canon<kRTNE>(o[e] * inv, o[e + 1] * inv);
-  }
+  o *= 1.f / l;
+  u32x2 y;
+  y[0] = pack2_bf16_canon<kRTNE>(o[0], o[1]);
+  y[1] = pack2_bf16_canon<kRTNE>(o[2], o[3]);
+  *reinterpret_cast<u32x2*>(a.out + 2 * (j.x * a.out_s[0] + t * a.out_s[1] + h * a.out_s[2] + lane * 4)) = y;
   if (a.lse && lane == 0) a.lse[((long long)j.x * a.q_len + t) * a.Hq + h] = kLn2 * (m + __builtin_amdgcn_logf(l));
 }
 
@@ -827,16 +861,18 @@ int launch(const DecodeArgs& a, const Plan& p, hipStream_t stream) {
   } else {
     using C = Shape<D, FP8, NT, RW, SHARED, true>;
     hipLaunchKernelGGL((gqa_decode_kernel<C>), dim3(p.grid), dim3(C::kThreads), 0, stream, a);
-    // Records of a row: as many as runs share a task, or two ends of a run. A wave takes
-    // four at once.
+    // Records of a row: as many as runs share a task, or two ends of a run. A group of
+    // lanes takes four at once.
+    constexpr int kMost = D == 256 ? 8 : 16, kGroups = kJoinThreads / (D / 4);
     const long long n = p.grid / p.tasks + 2, count = join_count(p);
     const int rows = p.row_blocks > 1 || p.rw > p.sets ? C::kRows : a.rows;
+    const auto blocks = [&](int per_row) { return dim3((unsigned)count, (rows * per_row + kGroups - 1) / kGroups); };
     if (n <= 4)
-      hipLaunchKernelGGL((gqa_join_kernel<D, NT, RW, 1>), dim3(count, (rows + 15) / 16), dim3(1024), 0, stream, a);
+      hipLaunchKernelGGL((gqa_join_kernel<D, NT, RW, 1>), blocks(1), dim3(kJoinThreads), 0, stream, a);
     else if (n <= 16)
-      hipLaunchKernelGGL((gqa_join_kernel<D, NT, RW, 4>), dim3(count, (rows + 3) / 4), dim3(1024), 0, stream, a);
+      hipLaunchKernelGGL((gqa_join_kernel<D, NT, RW, 4>), blocks(4), dim3(kJoinThreads), 0, stream, a);
     else
-      hipLaunchKernelGGL((gqa_join_kernel<D, NT, RW, 16>), dim3(count, rows), dim3(1024), 0, stream, a);
+      hipLaunchKernelGGL((gqa_join_kernel<D, NT, RW, kMost>), blocks(kMost), dim3(kJoinThreads), 0, stream, a);
   }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : (int)e;
