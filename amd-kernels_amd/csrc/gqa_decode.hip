@@ -57,6 +57,7 @@ struct DecodeArgs {
   int num_blocks, width, page_shift;
   float scale2;          // softmax scale * log2(e)
   float inv_g;           // 1 / G
+  double per_run;        // 1 / grid
 };
 
 // Workgroups of a CU. One 16-row tile of up to 128 dims fits three waves a SIMD
@@ -65,13 +66,16 @@ struct DecodeArgs {
 // 194; 32 requests of windows of 4, 16 rows a position, 4 kv heads: two 92 us, one 80.
 constexpr int per_cu(int D, int nt) { return D * nt <= 128 ? 3 : 1; }
 
+// Waves of a workgroup that takes a task whole.
+constexpr int whole_waves(int D, int nt) { return D * nt <= 128 ? 8 : 4; }
+
 // The kernel's shape: NT tiles of 16 rows for each wave, RW row sets; SHARED: of one
 // kv head, so that its rows are read by more than one wave.
 template <int D_, bool FP8_, int NT_, int RW_, bool SHARED_, bool SPLIT_>
 struct Shape {
   static constexpr int D = D_, NT = NT_, RW = RW_;
   static constexpr bool FP8 = FP8_, SPLIT = SPLIT_;
-  static constexpr int kWaves = !SPLIT && D * NT <= 128 ? 8 : 4, kThreads = 64 * kWaves;
+  static constexpr int kWaves = SPLIT ? 4 : whole_waves(D, NT), kThreads = 64 * kWaves;
   static constexpr int kGroups = kWaves / RW;           // of waves, by tokens
   static constexpr int kRow = FP8 ? D : 2 * D;          // bytes of a cached row
   static constexpr int kStep = 32;                      // tokens of a wave's step
@@ -389,19 +393,29 @@ __device__ __forceinline__ void compute_step(const DecodeArgs& a, Rows<C>& w, St
   if constexpr (!TAIL) load_v<C>(a, s, pg, next, head, lane);
 }
 
-// The runs: tile i of `total` belongs to run w where start(w) <= i < start(w + 1),
-// start(w) = floor(w * total / runs). No run is empty: there are at most `total`.
-__device__ __forceinline__ long long run_start(long long total, int runs, int w) {
-  return total / runs * w + total % runs * w / runs;
+// x / d of whole numbers below 2^52 (inv: 1 / d, rounded): the rounded product is at
+// most one off. A 64-bit division takes some 150 instructions, at a point that
+// everything waits for.
+__device__ __forceinline__ long long quotient(long long x, long long d, double inv) {
+  long long q = (long long)((double)x * inv);
+  const long long r = x - q * d;
+  q += r >= d ? 1 : 0;
+  q -= r < 0 ? 1 : 0;
+  return q;
 }
 
-// A workgroup's run, and the request in which its first tile lies with the number
-// of tiles before that.
+// The runs: tile i of `total` belongs to run w where start(w) <= i < start(w + 1),
+// start(w) = floor(w * total / runs). There are at most `total`, so none is empty.
 struct Run {
   long long total;
-  long long start, end;   // tiles of all tasks, in order
-  long long before;       // tiles before request b
-  int runs, b, len;       // and that request's length
+  int runs;               // the grid's workgroups, or `total` where that is less
+  double per_run;         // 1 / runs
+  long long start, end;   // this workgroup's run, in tiles of all tasks
+  long long before;       // tiles before request b, which holds its first tile
+  int b, len;             // and that request's length
+  __device__ __forceinline__ long long start_of(int w) const {
+    return runs == total ? w : quotient(w * total, runs, per_run);
+  }
 };
 // Every thread calls it. Requests are taken THREADS at a time, one for each thread, and
 // a prefix sum finds the one that holds the run's first tile.
@@ -435,10 +449,11 @@ __device__ Run find_run(const DecodeArgs& a, int wg, int grid) {
   Run run{};
   run.total = total = uniform(total * a.per);
   run.runs = (int)min((long long)grid, total);
+  run.per_run = a.per_run;
   run.b = a.B;
   if (wg >= run.runs) return run;
-  run.start = run_start(total, run.runs, wg);
-  run.end = run_start(total, run.runs, wg + 1);
+  run.start = uniform(run.start_of(wg));
+  run.end = uniform(run.start_of(wg + 1));
   long long base = 0;
   for (int b0 = 0, turn = 0; b0 < a.B; b0 += THREADS, turn ^= 1) {
     if (a.B > THREADS) {
@@ -548,7 +563,8 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
       x.before = run.before;
       x.len = run.len;
       x.tiles = tiles_of<C::kTile>(x.len);
-      x.task = uniform((int)((run.start - x.before) / x.tiles));
+      const long long in = run.start - x.before;
+      x.task = uniform(in >> 32 ? (int)(in / x.tiles) : (int)((uint32_t)in / (uint32_t)x.tiles));
       x.tile0 = uniform((int)(run.start - x.before - (long long)x.task * x.tiles));
       x.tile1 = uniform((int)min((long long)x.tiles, x.tile0 + (run.end - run.start)));
     }
@@ -692,10 +708,10 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
       int4 join{-1, 0, 0, 0};
       if (!whole) {
         const long long began = x.before + (long long)x.task * x.tiles;
-        int w0 = (int)(began * run.runs / run.total);
-        while (run_start(run.total, run.runs, w0) > began) --w0;
-        while (run_start(run.total, run.runs, w0 + 1) <= began) ++w0;
-        join = int4{x.b, x.task, 2 * w0 + (run_start(run.total, run.runs, w0) == began ? 0 : 1), wg};
+        int w0 = min((int)((double)began / (double)run.total * run.runs), wg);
+        while (run.start_of(w0) > began) --w0;
+        while (run.start_of(w0 + 1) <= began) ++w0;
+        join = int4{x.b, x.task, 2 * w0 + (run.start_of(w0) == began ? 0 : 1), wg};
       }
       if (a.joins_by_task)
         a.joins[x.b * a.per + x.task] = join;
@@ -821,9 +837,14 @@ struct Plan {
   long long tasks;
 };
 constexpr int kCus = 256;
-// Up to this many tokens in the longest request a call runs a workgroup for each
-// task, without the plan's reads and the second launch.
-constexpr long long kShort = 512;
+// Whether a workgroup takes each task whole, without the plan's reads and the second
+// launch: where the longest request is two steps of each wave, or four where there are
+// tasks enough for a quarter of the CUs. One request of 200 tokens (8 kv heads) 7.3 us,
+// shared out 9.0; of 1000 14.1 and 9.5; 64 of up to 500 16.3 and 25, of up to 1000
+// 42.3 and 50; 64 of up to 2000 the same.
+inline bool short_call(long long most, long long tasks, int D, int nt) {
+  return most <= (tasks >= kCus / 4 ? 4 : 2) * 32 * whole_waves(D, nt);
+}
 
 // A K cache whose tokens hold their heads side by side (strides: as the launcher's).
 inline bool token_major(const long long* strides) { return strides[8] > strides[7]; }
@@ -833,7 +854,7 @@ inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int wi
   const long long sets = (rows + 16 * p->nt - 1) / (16 * p->nt);
   p->sets = sets == 1 ? 1 : sets == 2 ? 2 : 4;
   p->rw = p->sets;
-  p->split = p->sets > 1 || most > kShort;
+  p->split = p->sets > 1 || !short_call(most, (long long)B * Hkv, D, p->nt);
   // Rows of neighbouring heads: four waves that read them together read whole lines
   // and neighbouring ones.
   if (p->split && by_token)
@@ -964,6 +985,7 @@ int launch_gqa_decode_paged(const void* q, const void* k_cache, const void* v_ca
   a.page_shift = __builtin_ctz(page);
   a.scale2 = scale * kLog2e;
   a.inv_g = 1.f / (float)a.G;
+  a.per_run = 1.0 / (double)p.grid;
   return k_scale ? dispatch<true>(a, p, head_dim, (hipStream_t)stream) : dispatch<false>(a, p, head_dim, (hipStream_t)stream);
 }
 
