@@ -104,8 +104,8 @@ __global__ __launch_bounds__(kThreads) void gqa_write_kernel(const RowsArgs a) {
   }
   if (!live) return;
   constexpr int kElem = FP8 ? 1 : 2;
-  *reinterpret_cast<u32x4*>(a.kc.base + row_at(a.kc, slot, a.page_shift, head) * kElem + 16 * c) = ko;
-  *reinterpret_cast<u32x4*>(a.vc.base + row_at(a.vc, slot, a.page_shift, head) * kElem + 16 * c) = vo;
+  __builtin_nontemporal_store(ko, reinterpret_cast<u32x4*>(a.kc.base + row_at(a.kc, slot, a.page_shift, head) * kElem + 16 * c));
+  __builtin_nontemporal_store(vo, reinterpret_cast<u32x4*>(a.vc.base + row_at(a.vc, slot, a.page_shift, head) * kElem + 16 * c));
   if (FP8 && c == 0) {
     a.kc.scale[scale_at(a.kc, slot, a.page_shift, head)] = ks;
     a.vc.scale[scale_at(a.vc, slot, a.page_shift, head)] = vs;
