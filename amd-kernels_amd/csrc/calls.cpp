@@ -636,7 +636,7 @@ PyObject* gqa_decode(PyObject*, PyObject* const* x, Py_ssize_t n) {
           !at::isTensorSubclassLike(table) && !table.is_neg() && table.dim() == 2 && table.size(0) == B &&
           table.size(1) >= 1 && (table.size(1) == 1 || table.stride(1) == 1));
     const int width = as_int(table.size(1));
-    plain((int64_t)width * c.page <= ((int64_t)1 << 31) - 64);
+    plain((int64_t)width * c.page <= ((int64_t)1 << 31) - 4096);
     const float scale = x[5] == Py_None ? (float)(1.0 / std::sqrt((double)c.D)) : float_arg(x[5]);
     Tensor out, lse;
     if (x[8] != Py_None) {
@@ -660,7 +660,7 @@ PyObject* gqa_decode(PyObject*, PyObject* const* x, Py_ssize_t n) {
       }
       std::copy(c.strides, c.strides + 10, st + 6);
       st[16] = table.stride(0);
-      const size_t need = abi.moonmath_gqa_decode_workspace(B, q_len, Hq, c.heads, c.D, c.page, width, st);
+      const size_t need = abi.moonmath_gqa_decode_workspace(B, q_len, Hq, c.heads, c.D, c.page, width, c.ks.defined(), st);
       const Tensor ws = need ? bytes(need, q) : Tensor();
       check_rc(abi.launch_gqa_decode_paged(q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), ptr_or_null(c.ks),
                                            ptr_or_null(c.vs), out.data_ptr(), ptr_or_null(lse), lens.data_ptr(),

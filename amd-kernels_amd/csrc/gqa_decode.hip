@@ -6,13 +6,13 @@
 // zeros where that leaves no token, with lse = ln sum_j exp(scale * q . k_j).
 //
 // A task is one request and RW "row sets" of 16 * NT query rows (row t * G + g of a kv
-// head): those of one kv head, or of neighbouring ones. The tasks' tiles of tokens, in
+// head): those of one kv head, or of neighbouring ones. The tasks' steps of 32 tokens, in
 // order, are cut into equal runs, one for each workgroup; a task that a cut divides
 // leaves fp32 records (O, m, l) that a second kernel joins. So the work is even whatever
 // the lengths are, they are read on the device, and the workspace depends on neither.
 //
 // Within a workgroup RW waves take a row set each and the same tokens, and WAVES / RW
-// such groups of waves take the steps of 32 tokens in turn, each with its own running
+// such groups of waves take the steps in turn, each with its own running
 // maximum and sum (one pass over the data); they are joined in LDS at the task's end.
 //
 // No operand passes through LDS. 16x16x32 MFMAs compute S^T = K Q^T and
@@ -32,9 +32,10 @@
 namespace mm {
 namespace gqa {
 
+constexpr int kStep = 32;  // tokens of a wave's step
 constexpr int kMaxQLen = 8;
 constexpr int kMaxHeads = 1 << 16;
-constexpr long long kMaxTokens = (1LL << 31) - 64;  // of a request's table
+constexpr long long kMaxTokens = (1LL << 31) - 4096;  // of a request's table
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -66,6 +67,10 @@ struct DecodeArgs {
 // 194; 32 requests of windows of 4, 16 rows a position, 4 kv heads: two 92 us, one 80.
 constexpr int per_cu(int D, int nt) { return D * nt <= 128 ? 3 : 1; }
 
+// What a task's start and end cost a workgroup, as steps: about 4 us, in which one of
+// three on a CU streams 32 KB, and half a step of each group of waves that has none.
+constexpr int lead_steps(int D, bool fp8, int rw) { return 4 / rw / 2 + 512 / (fp8 ? D : 2 * D); }
+
 // Waves of a workgroup that takes a task whole.
 constexpr int whole_waves(int D, int nt) { return D * nt <= 128 ? 8 : 4; }
 
@@ -78,13 +83,12 @@ struct Shape {
   static constexpr int kWaves = SPLIT ? 4 : whole_waves(D, NT), kThreads = 64 * kWaves;
   static constexpr int kGroups = kWaves / RW;           // of waves, by tokens
   static constexpr int kRow = FP8 ? D : 2 * D;          // bytes of a cached row
-  static constexpr int kStep = 32;                      // tokens of a wave's step
-  static constexpr int kTile = kStep * kGroups;         // tokens of a tile
   static constexpr int kRows = 16 * NT * RW;            // of a task
   static constexpr int kPerCu = SPLIT ? per_cu(D, NT) : 2;
   static constexpr bool kOnce = !SHARED_ && SPLIT && !(D == 256 && !FP8);  // streamed past the caches
   static constexpr int kKLoads = kRow / 64;             // 16-byte loads of K per lane and 16 tokens
   static constexpr int kVWords = kRow / 64;             // dwords of V per lane and token
+  static constexpr int kLead = SPLIT ? lead_steps(D, FP8, RW) : 0;
 };
 
 __device__ __forceinline__ float xor16_max(float x) {
@@ -107,12 +111,7 @@ __device__ __forceinline__ int clamped(const DecodeArgs& a, int n) {
   return n < 0 ? 0 : (n > most ? (int)most : n);
 }
 __device__ __forceinline__ int len_of(const DecodeArgs& a, int b) { return clamped(a, ((ConstInts)(uintptr_t)a.seq_lens)[b]); }
-template <int TILE>
-__device__ __forceinline__ int tiles_of(int len) {
-  constexpr int kShift = __builtin_ctz(TILE);
-  static_assert(TILE == 1 << kShift, "tiles are powers of two");
-  return (len >> kShift) + ((len & (TILE - 1)) != 0);
-}
+__host__ __device__ __forceinline__ int steps_of(int len) { return (len >> 5) + ((len & 31) != 0); }
 
 __device__ __forceinline__ long long uniform(long long x) {
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
@@ -396,7 +395,7 @@ __device__ __forceinline__ void compute_step(const DecodeArgs& a, Rows<C>& w, St
 // x / d of whole numbers below 2^52 (inv: 1 / d, rounded): the rounded product is at
 // most one off. A 64-bit division takes some 150 instructions, at a point that
 // everything waits for.
-__device__ __forceinline__ long long quotient(long long x, long long d, double inv) {
+__host__ __device__ __forceinline__ long long quotient(long long x, long long d, double inv) {
   long long q = (long long)((double)x * inv);
   const long long r = x - q * d;
   q += r >= d ? 1 : 0;
@@ -404,32 +403,70 @@ __device__ __forceinline__ long long quotient(long long x, long long d, double i
   return q;
 }
 
-// The runs: tile i of `total` belongs to run w where start(w) <= i < start(w + 1),
-// start(w) = floor(w * total / runs). There are at most `total`, so none is empty.
+// The runs: the tasks lie one behind the other, each as long as its steps and `lead`
+// places more in front for its own cost; run w has the places from start(w) = floor(w *
+// total / runs) up to start(w + 1). Where there are not steps enough for all workgroups,
+// a task is as long as its steps in whole rounds of the groups of waves, and a run a round.
 struct Run {
   long long total;
-  int runs;               // the grid's workgroups, or `total` where that is less
+  int runs;               // the grid's workgroups, or as many as give each group of waves a step
+  int lead, pad, snap;
   double per_run;         // 1 / runs
-  long long start, end;   // this workgroup's run, in tiles of all tasks
-  long long before;       // tiles before request b, which holds its first tile
+  long long start, end;   // this workgroup's run
+  long long before;       // places before request b, in which it starts
   int b, len;             // and that request's length
-  __device__ __forceinline__ long long start_of(int w) const {
-    return runs == total ? w : quotient(w * total, runs, per_run);
+  __host__ __device__ __forceinline__ long long start_of(int w) const { return quotient(w * total, runs, per_run); }
+  __host__ __device__ __forceinline__ void by_rounds(int groups) {
+    lead = 0;
+    pad = groups - 1;  // groups: a power of two
+  }
+  __host__ __device__ __forceinline__ void by_cost(int steps) {
+    lead = steps;
+    pad = 0;
+  }
+  __host__ __device__ __forceinline__ int places_of(int steps) const { return (steps + lead + pad) & ~pad; }
+  __host__ __device__ __forceinline__ void lay_out(long long places, int grid, double per_grid, int groups) {
+    total = places;
+    const long long most = (total + groups - 1) / groups;
+    runs = grid < most ? grid : (int)most;
+    per_run = runs == grid ? per_grid : 1.0 / (double)runs;
+    snap = pad ? 0 : total >= 2LL * groups * runs ? groups : (int)(total / 2) / runs;
+  }
+  // The steps of a task of `steps` that lie before its place v: a run's border near the
+  // task's start or end is moved there, so that it costs no segment of its own.
+  __host__ __device__ __forceinline__ int cut(long long v, int steps) const {
+    const long long r = v - lead;
+    const int late = snap < steps >> 1 ? snap : steps >> 1;
+    return r < least_cut(steps) ? 0 : r >= steps - late ? steps : (int)r;
+  }
+  __host__ __device__ __forceinline__ int least_cut(int steps) const {
+    const int soon = snap < (steps + 1) >> 1 ? snap : (steps + 1) >> 1;
+    return soon > 1 ? soon : 1;
+  }
+  // The run that holds the beginning of a task that starts at place `at` and has been
+  // cut: the last whose start is not yet cut into the task. `guess`: a later one.
+  __host__ __device__ __forceinline__ int holder(long long at, int steps, int guess) const {
+    const long long first = at + lead + least_cut(steps);
+    int w = (int)((double)first / (double)total * runs);
+    w = w < guess ? w : guess - 1;
+    while (start_of(w) >= first) --w;
+    while (start_of(w + 1) < first) ++w;
+    return w;
   }
 };
 // Every thread calls it. Requests are taken THREADS at a time, one for each thread, and
-// a prefix sum finds the one that holds the run's first tile.
-template <int THREADS, int TILE>
+// a prefix sum finds the one that holds the run's first place.
+template <int THREADS, int GROUPS, int LEAD>
 __device__ Run find_run(const DecodeArgs& a, int wg, int grid) {
   constexpr int kWaves = THREADS / 64;
   __shared__ int sh_sum[2][kWaves];
   __shared__ long long sh_found[3];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  // A wave's 64 requests have fewer than 2^32 tiles; sums over waves are 64 bits.
-  static_assert(TILE >= 32, "64 requests of at most kMaxTokens");
+  // A wave's 64 requests have fewer than 2^32 places; sums over waves are 64 bits.
+  Run run{};
   const auto group = [&](int b0, int turn, int& len, int& n, int& incl, long long& ahead, long long& sum) {
     len = b0 + tid < a.B ? clamped(a, a.seq_lens[b0 + tid]) : 0;
-    n = tiles_of<TILE>(len);
+    n = len > 0 ? run.places_of(steps_of(len)) : 0;
     incl = wave_incl_scan(n);
     if (lane == 63) sh_sum[turn][wave] = incl;
     __syncthreads();
@@ -441,15 +478,23 @@ __device__ Run find_run(const DecodeArgs& a, int wg, int grid) {
     }
   };
   int len, n, incl;
-  long long ahead, sum, total = 0;
-  for (int b0 = 0, turn = 0; b0 < a.B; b0 += THREADS, turn ^= 1) {
-    group(b0, turn, len, n, incl, ahead, sum);
-    total += sum;
+  long long ahead, sum, total;
+  if constexpr (GROUPS > 1)
+    run.by_rounds(GROUPS);
+  else
+    run.by_cost(LEAD);
+  while (true) {
+    total = 0;
+    for (int b0 = 0, turn = 0; b0 < a.B; b0 += THREADS, turn ^= 1) {
+      group(b0, turn, len, n, incl, ahead, sum);
+      total += sum;
+    }
+    total = uniform(total * a.per);
+    if (run.pad == 0 || total <= (long long)grid * GROUPS) break;
+    run.by_cost(LEAD);
+    __syncthreads();
   }
-  Run run{};
-  run.total = total = uniform(total * a.per);
-  run.runs = (int)min((long long)grid, total);
-  run.per_run = a.per_run;
+  run.lay_out(total, grid, a.per_run, GROUPS);
   run.b = a.B;
   if (wg >= run.runs) return run;
   run.start = uniform(run.start_of(wg));
@@ -488,9 +533,9 @@ __device__ __forceinline__ int position(const DecodeArgs& a, int r) { return (in
 
 // The part of a task that a workgroup takes, all of it wave-uniform.
 struct Segment {
-  long long before;           // tiles before request b
-  int b, task, len, tiles;    // the request's length and a task's tiles
-  int tile0, tile1;
+  long long before, start;    // places before request b, and before the task
+  int b, task, len, steps;    // the request's length and a task's steps
+  int step0, step1;           // its part: steps [step0, step1)
   int head0, block;           // the task's first kv head and block of its rows
 };
 template <class C>
@@ -500,14 +545,33 @@ __device__ __forceinline__ void place(const DecodeArgs& a, Segment& x) {
   x.head0 = a.sets == C::RW ? group : a.sets * 2 == C::RW ? group * 2 : group * 4;
 }
 
+// The next task's part in the run; false where it has none.
+template <class C>
+__device__ __forceinline__ bool next_task(const DecodeArgs& a, const Run& run, Segment& x) {
+  x.start += run.places_of(x.steps);
+  if (x.start >= run.end) return false;
+  if (++x.task == a.per) {
+    x.task = 0;
+    x.before = x.start;
+    do {
+      if (++x.b >= a.B) return false;
+      x.len = len_of(a, x.b);
+    } while (x.len == 0);
+    x.steps = steps_of(x.len);
+  }
+  x.step0 = 0;
+  x.step1 = uniform(run.cut(run.end - x.start, x.steps));
+  return x.step1 > 0;
+}
+
 // A wave's first loads for a segment: its query rows and its first step.
 template <class C>
 __device__ __forceinline__ void begin(const DecodeArgs& a, const Segment& x, Rows<C>& w, Step<C>& s, int rw, int tg,
                                       int lane) {
   constexpr int NT = C::NT;
-  const int st = x.tile0 * C::kGroups + tg, n = lane & 15, g = lane >> 4;
+  const int st = x.step0 + tg, n = lane & 15, g = lane >> 4;
   const ConstInts table = (ConstInts)(uintptr_t)(a.table + (long long)x.b * a.table_s);
-  const Pages<C> pg = step_pages<C>(a, table, st * C::kStep);
+  const Pages<C> pg = step_pages<C>(a, table, st * kStep);
   int head, row0;
   row_of<NT>(a, x.head0, x.block, rw * 16 * NT, head, row0);
 #pragma unroll
@@ -529,13 +593,13 @@ __device__ __forceinline__ void begin(const DecodeArgs& a, const Segment& x, Row
   // K before V here as in the loop: the compiler's wait for K there counts the loads
   // that may have been issued since on every way into it.
   sched_fence();
-  load_k<C>(a, s, pg, st * C::kStep, head, lane);
+  load_k<C>(a, s, pg, st * kStep, head, lane);
   sched_fence();
-  load_v<C>(a, s, pg, st * C::kStep, head, lane);
+  load_v<C>(a, s, pg, st * kStep, head, lane);
   sched_fence();
 }
 
-// SPLIT: the workgroup takes its run of all tasks' tiles. Otherwise a whole task:
+// SPLIT: the workgroup takes its run of all tasks' steps. Otherwise a whole task:
 // nothing is planned, and the first step is loaded before the request's length is there.
 template <class C>
 __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(const DecodeArgs a) {
@@ -555,25 +619,26 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
   if constexpr (SPLIT) {
     grid = gridDim.x;
     wg = xcd_remap(blockIdx.x, grid);
-    run = find_run<kThreads, C::kTile>(a, wg, grid);
+    run = find_run<kThreads, C::kGroups, C::kLead>(a, wg, grid);
     if (!a.joins_by_task && tid == 0) a.joins[wg] = int4{-1, 0, 0, 0};
     more = run.start < run.end;
     if (more) {
       x.b = run.b;
       x.before = run.before;
       x.len = run.len;
-      x.tiles = tiles_of<C::kTile>(x.len);
+      x.steps = steps_of(x.len);
       const long long in = run.start - x.before;
-      x.task = uniform(in >> 32 ? (int)(in / x.tiles) : (int)((uint32_t)in / (uint32_t)x.tiles));
-      x.tile0 = uniform((int)(run.start - x.before - (long long)x.task * x.tiles));
-      x.tile1 = uniform((int)min((long long)x.tiles, x.tile0 + (run.end - run.start)));
+      const int places = run.places_of(x.steps);
+      x.task = uniform(in >> 32 ? (int)(in / places) : (int)((uint32_t)in / (uint32_t)places));
+      x.start = x.before + (long long)x.task * places;
+      x.step0 = uniform(run.cut(run.start - x.start, x.steps));
+      x.step1 = uniform(run.cut(run.end - x.start, x.steps));
+      more = x.step0 < x.step1 || (x.step0 == x.steps && next_task<C>(a, run, x));
     }
   } else {
     x.b = blockIdx.x;
     x.task = blockIdx.y;
   }
-  long long at = run.start;
-  bool first = true;
   while (more) {
     place<C>(a, x);
     Rows<C> w;
@@ -581,7 +646,7 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
     begin<C>(a, x, w, s, rw, tg, lane);
     if constexpr (!SPLIT) {
       x.len = len_of(a, x.b);
-      x.tile1 = x.tiles = tiles_of<C::kTile>(x.len);
+      x.step1 = x.steps = steps_of(x.len);
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -599,35 +664,35 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
       const ConstInts table = (ConstInts)(uintptr_t)(a.table + (long long)x.b * a.table_s);
       int head, row0;
       row_of<NT>(a, x.head0, x.block, rw * 16 * NT, head, row0);
-      int st = x.tile0 * C::kGroups + tg;
-      const int s_end = min(x.tile1 * C::kGroups, tiles_of<C::kStep>(x.len));
+      int st = x.step0 + tg;
+      const int s_end = x.step1;
       if (st < s_end && row0 < a.rows) {
         const int s_last = st + (s_end - 1 - st) / C::kGroups * C::kGroups;
         const int seen = x.len - a.q_len + 1;
-        const int s_full = seen > 0 ? seen / C::kStep : 0;
+        const int s_full = seen > 0 ? seen / kStep : 0;
         int next = min(st + C::kGroups, s_last);
-        Pages<C> pg = step_pages<C>(a, table, next * C::kStep);
+        Pages<C> pg = step_pages<C>(a, table, next * kStep);
         for (; st <= s_last && st < s_full; st += C::kGroups) {
           const int after = min(next + C::kGroups, s_last);
-          const Pages<C> pa = step_pages<C>(a, table, after * C::kStep);
-          compute_step<C, false>(a, w, s, st * C::kStep, x.len, pg, next * C::kStep, head, lane);
+          const Pages<C> pa = step_pages<C>(a, table, after * kStep);
+          compute_step<C, false>(a, w, s, st * kStep, x.len, pg, next * kStep, head, lane);
           pg = pa;
           next = after;
         }
         while (st <= s_last) {
-          compute_step<C, true>(a, w, s, st * C::kStep, x.len, pg, 0, head, lane);
+          compute_step<C, true>(a, w, s, st * kStep, x.len, pg, 0, head, lane);
           st += C::kGroups;
           if (C::kGroups > 1 || st > s_last) break;  // a wave of several has one such step
-          pg = step_pages<C>(a, table, st * C::kStep);
-          load_k<C>(a, s, pg, st * C::kStep, head, lane);
-          load_v<C>(a, s, pg, st * C::kStep, head, lane);
+          pg = step_pages<C>(a, table, st * kStep);
+          load_k<C>(a, s, pg, st * kStep, head, lane);
+          load_v<C>(a, s, pg, st * kStep, head, lane);
         }
       }
     }
 
     // Join the waves. The barriers wait for LDS alone.
-    const bool whole = !SPLIT || (x.tile0 == 0 && x.tile1 == x.tiles);
-    const int rec = 2 * wg + (first ? 0 : 1);
+    const bool whole = !SPLIT || (x.step0 == 0 && x.step1 == x.steps);
+    const int rec = 2 * wg + (x.step0 == 0 ? 1 : 0);  // a run has one part that begins a task, and one that does not
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       w.l[nt] = xor32_sum(xor16_sum(w.l[nt]));
@@ -702,39 +767,16 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
       lds_reads_done_barrier();
     }
     if constexpr (!SPLIT) return;
-    if (x.tile1 == x.tiles && tid == 0) {
-      // The task ends in this run. Where it began in an earlier one: that run, and which
-      // of its two records holds the beginning (its first segment's, or its last's).
+    if (x.step1 == x.steps && tid == 0) {
+      // The task ends in this run: which others hold it.
       int4 join{-1, 0, 0, 0};
-      if (!whole) {
-        const long long began = x.before + (long long)x.task * x.tiles;
-        int w0 = min((int)((double)began / (double)run.total * run.runs), wg);
-        while (run.start_of(w0) > began) --w0;
-        while (run.start_of(w0 + 1) <= began) ++w0;
-        join = int4{x.b, x.task, 2 * w0 + (run.start_of(w0) == began ? 0 : 1), wg};
-      }
+      if (!whole) join = int4{x.b, x.task, run.holder(x.start, x.steps, wg), wg};
       if (a.joins_by_task)
         a.joins[x.b * a.per + x.task] = join;
       else if (!whole)
         a.joins[wg] = join;  // of the first segment only: one for each run
     }
-    first = false;
-    at += x.tile1 - x.tile0;
-    more = at < run.end;
-    x.tile0 = 0;
-    if (more && ++x.task == a.per) {
-      x.task = 0;
-      do {
-        x.before += (long long)x.tiles * a.per;
-        if (++x.b >= a.B) {
-          more = false;
-          break;
-        }
-        x.len = len_of(a, x.b);
-        x.tiles = tiles_of<C::kTile>(x.len);
-      } while (x.tiles == 0);
-    }
-    x.tile1 = (int)min((long long)x.tiles, run.end - at);
+    more = x.step1 == x.steps && next_task<C>(a, run, x);
   }
 
   // Requests without a token: zeros.
@@ -769,7 +811,7 @@ __global__ __launch_bounds__(kJoinThreads) void gqa_join_kernel(const DecodeArgs
   int head, R;
   row_of<NT>(a, group * (RW / a.sets), block, row, head, R);
   const bool live = row < kRows && R < a.rows;  // what other rows join is not stored
-  const int n = j.w - (j.z >> 1) + 1;
+  const int n = j.w - j.z + 1;
   float m = kNegFltMax, l = 0.f;
   f32x4 o{0.f, 0.f, 0.f, 0.f};
   for (int i0 = sub; live && i0 < n; i0 += 4 * PER_ROW) {
@@ -778,7 +820,7 @@ __global__ __launch_bounds__(kJoinThreads) void gqa_join_kernel(const DecodeArgs
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int i = min(i0 + u * PER_ROW, n - 1);
-      const long long r = (long long)(i == 0 ? j.z : 2 * ((j.z >> 1) + i)) * kRows + row;
+      const long long r = (long long)(2 * (j.z + i) + (i == 0 ? 1 : 0)) * kRows + row;
       pm[u] = a.rec_ml[2 * r];
       pl[u] = a.rec_ml[2 * r + 1];
       po[u] = *reinterpret_cast<const f32x4*>(a.rec_o + r * D + lane * 4);
@@ -833,7 +875,7 @@ __global__ __launch_bounds__(kJoinThreads) void gqa_join_kernel(const DecodeArgs
 struct Plan {
   int nt, rw, sets;          // 16-row tiles of a wave, row sets of a task, and of those one kv head's
   int row_blocks, per;       // tasks of a kv head's rows, and of a request
-  int grid, split;           // workgroups; whether they share the tiles evenly or take a task each
+  int grid, split;           // workgroups; whether they share the steps evenly or take a task each
   long long tasks;
 };
 constexpr int kCus = 256;
@@ -848,7 +890,8 @@ inline bool short_call(long long most, long long tasks, int D, int nt) {
 
 // A K cache whose tokens hold their heads side by side (strides: as the launcher's).
 inline bool token_major(const long long* strides) { return strides[8] > strides[7]; }
-inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int width, bool by_token, Plan* p) {
+inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int width, bool fp8, bool by_token,
+                      Plan* p) {
   const long long rows = (long long)(Hq / Hkv) * q_len, most = (long long)page * width;
   p->nt = rows <= 16 || D == 256 ? 1 : 2;
   const long long sets = (rows + 16 * p->nt - 1) / (16 * p->nt);
@@ -864,9 +907,11 @@ inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int wi
   if (per > 65535) return false;
   p->per = (int)per;
   p->tasks = B * per;
-    const long long tile = 32LL * (4 / p->rw), tiles = (most + tile - 1) / tile, slots = per_cu(D, p->nt) * kCus;
-  p->grid = (int)(p->tasks >= slots || p->tasks * tiles >= slots ? slots : p->tasks * tiles);
-  return p->tasks <= INT_MAX;
+    const long long steps = (most + 31) / 32, slots = per_cu(D, p->nt) * kCus;
+  const long long places = steps + lead_steps(D, fp8, p->rw);
+  const long long runs = (p->tasks * places * p->rw + 3) / 4;  // of a step for each group of waves
+  p->grid = (int)(runs < slots ? runs : slots);
+  return p->tasks <= INT_MAX && p->tasks * places < 1LL << 42;  // quotient()'s range
 }
 inline size_t record_bytes(const Plan& p, int D) { return (size_t)2 * p.grid * 16 * p.nt * p.rw * (D + 2) * 4; }
 // One entry for each task or run, whichever are fewer.
@@ -931,12 +976,57 @@ inline int check_sizes(int B, int q_len, int Hq, int Hkv, int D, int page, int w
 extern "C" {
 
 size_t moonmath_gqa_decode_workspace(int B, int q_len, int Hq, int Hkv, int head_dim, int page, int max_blocks,
-                                     const long long* strides) {
+                                     int fp8, const long long* strides) {
   using namespace mm::gqa;
   Plan p;
   if (B == 0 || !strides || check_sizes(B, q_len, Hq, Hkv, head_dim, page, max_blocks) != 0) return 0;
-  if (!plan_call(B, q_len, Hq, Hkv, head_dim, page, max_blocks, token_major(strides), &p) || !p.split) return 0;
+  if (!plan_call(B, q_len, Hq, Hkv, head_dim, page, max_blocks, fp8 != 0, token_major(strides), &p) || !p.split) return 0;
   return record_bytes(p, head_dim) + (size_t)join_count(p) * sizeof(int4);
+}
+
+int moonmath_gqa_decode_split(int B, const int* lens, int q_len, int Hq, int Hkv, int head_dim, int page,
+                              int max_blocks, int fp8, const long long* strides, int* segments, int max_segments) {
+  using namespace mm::gqa;
+  const int rc = check_sizes(B, q_len, Hq, Hkv, head_dim, page, max_blocks);
+  if (rc != 0) return rc;
+  if (!lens || !strides || (!segments && max_segments > 0)) return -6;
+  Plan p;
+  if (B == 0) return 0;
+  if (!plan_call(B, q_len, Hq, Hkv, head_dim, page, max_blocks, fp8 != 0, token_major(strides), &p)) return -8;
+  if (!p.split) return 0;
+  const int lead = lead_steps(head_dim, fp8 != 0, p.rw);
+  Run run{};
+  const auto places = [&] {
+    long long sum = 0;
+    for (int b = 0; b < B; ++b) sum += lens[b] > 0 ? run.places_of(steps_of(lens[b])) : 0;
+    return sum * p.per;
+  };
+  const int groups = 4 / p.rw;
+  run.by_rounds(groups);
+  if (groups == 1 || places() > (long long)p.grid * groups) run.by_cost(lead);
+  run.lay_out(places(), p.grid, 1.0 / p.grid, groups);
+  long long n = 0;
+  long long before = 0;
+  for (int b = 0; b < B; ++b) {
+    if (lens[b] <= 0) continue;
+    const int steps = steps_of(lens[b]), length = run.places_of(steps);
+    for (int task = 0; task < p.per; ++task, before += length) {
+      // The runs that start within the task's places, and the one before them.
+      int w = (int)((double)before / (double)run.total * run.runs);
+      while (w > 0 && run.start_of(w) > before) --w;
+      while (w + 1 < run.runs && run.start_of(w + 1) <= before) ++w;
+      for (; w < run.runs && run.start_of(w) < before + length; ++w) {
+        const int s0 = run.cut(run.start_of(w) - before, steps), s1 = run.cut(run.start_of(w + 1) - before, steps);
+        if (s0 >= s1) continue;
+        const int part[8] = {w, b, task, s0, s1, s0 == 0 && s1 == steps ? -1 : 2 * w + (s0 == 0 ? 1 : 0),
+                             s0 > 0 && s1 == steps ? run.holder(before, steps, w) : -1, steps};
+        for (int i = 0; i < 8; ++i)
+          if (n < max_segments) segments[8 * n + i] = part[i];
+        ++n;
+      }
+    }
+  }
+  return n > INT_MAX ? -8 : (int)n;
 }
 
 int launch_gqa_decode_paged(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
@@ -956,7 +1046,7 @@ int launch_gqa_decode_paged(const void* q, const void* k_cache, const void* v_ca
   const long long widest = 1LL << 26;
   if (a.k.row_s < 0 || a.v.row_s < 0 || a.k.row_s > widest || a.v.row_s > widest) return -9;
   Plan p;
-  if (!plan_call(B, q_len, Hq, Hkv, head_dim, page, max_blocks, token_major(strides), &p)) return -8;
+  if (!plan_call(B, q_len, Hq, Hkv, head_dim, page, max_blocks, k_scale != nullptr, token_major(strides), &p)) return -8;
   if (p.split && !workspace) return -6;
   a.q = (const char*)q;
   a.out = (char*)out;

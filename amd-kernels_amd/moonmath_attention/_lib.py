@@ -73,7 +73,8 @@ SIGNATURES.update({
     "launch_gqa_kv_read": (_i, [_p, _p, _p, _p, _p, _p, _p, _ll, _i, _i, _i, _i, _llp, _p]),
     "launch_gqa_decode_paged": (
         _i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _llp, _f, _p, _p]),
-    "moonmath_gqa_decode_workspace": (_sz, [_i, _i, _i, _i, _i, _i, _i, _llp]),
+    "moonmath_gqa_decode_workspace": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _llp]),
+    "moonmath_gqa_decode_split": (_i, [_i, _ip, _i, _i, _i, _i, _i, _i, _i, _llp, _ip, _i]),
     "launch_rope_axes": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _llp, _p]),
 })
 

@@ -31,7 +31,7 @@ _FP8 = torch.float8_e4m3fn
 _DIMS = (64, 128, 256)
 _MAX_Q_LEN = 8
 _MAX_HEADS = 1 << 16
-_MAX_TOKENS = (1 << 31) - 64
+_MAX_TOKENS = (1 << 31) - 4096
 _MAX_ROW_STRIDE = 1 << 26
 
 
@@ -198,7 +198,7 @@ def gqa_decode_paged(q, k_cache, v_cache, seq_lens, block_table, *, scale=None, 
     if res is not None:
         return res
     who = "gqa_decode_paged"
-    nb, heads, page, D, _ = _check_cache(k_cache, v_cache, k_scale, v_scale, who, False)
+    nb, heads, page, D, fp8 = _check_cache(k_cache, v_cache, k_scale, v_scale, who, False)
     ck.tensor(q, "q", who, torch.bfloat16)
     if q.dim() not in (3, 4) or q.shape[-1] != D:
         raise ValueError(f"{who}: q must be [B, Hq, {D}] or [B, q_len, Hq, {D}], got {list(q.shape)}")
@@ -216,7 +216,7 @@ def gqa_decode_paged(q, k_cache, v_cache, seq_lens, block_table, *, scale=None, 
     if block_table.dim() != 2 or block_table.shape[0] != B or block_table.shape[1] < 1:
         raise ValueError(f"{who}: block_table must be [B, max_blocks] with B = {B}, got {list(block_table.shape)}")
     if block_table.shape[1] * page > _MAX_TOKENS:
-        raise ValueError(f"{who}: a request's table must hold at most 2^31 - 64 tokens")
+        raise ValueError(f"{who}: a request's table must hold at most 2^31 - 4096 tokens")
     if block_table.shape[1] > 1 and block_table.stride(1) != 1:
         raise ValueError(f"{who}: block_table's last dim must be contiguous")
     if out is not None:
@@ -241,7 +241,7 @@ def gqa_decode_paged(q, k_cache, v_cache, seq_lens, block_table, *, scale=None, 
                        *_cache_strides(v_cache, v_scale), block_table.stride(0))
     p = _lib.ptr
     with torch.cuda.device(dev):
-        nbytes = _lib.lib.moonmath_gqa_decode_workspace(B, q_len, Hq, heads, D, page, width, strides)
+        nbytes = _lib.lib.moonmath_gqa_decode_workspace(B, q_len, Hq, heads, D, page, width, int(fp8), strides)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
         _run("launch_gqa_decode_paged", p(q), p(k_cache), p(v_cache), p(k_scale), p(v_scale), p(out), p(lse),
              p(seq_lens), p(block_table), B, q_len, Hq, heads, D, nb, page, width, strides, scale, p(ws),

@@ -277,7 +277,7 @@ int moonmath_pack_bf16(const void* in, void* out, int n, int round_mode, void* s
  * scale head}. page: rows of a block, a power of two, at least 16.
  * Codes: -2 head_dim, -3 heads, -4 sizes, -5 page or pairs, -6 null pointer,
  * -8 grid overflow, -9 row stride above 2^26, -11 bad block-table or pool geometry
- * (a request's table holds at most 2^31 - 64 tokens).
+ * (a request's table holds at most 2^31 - 4096 tokens).
  * ------------------------------------------------------------------------- */
 
 /* Rows of new tokens into their slots (block * page + row; int32, outside
@@ -311,7 +311,16 @@ int launch_gqa_decode_paged(const void* q, const void* k_cache, const void* v_ca
                             int B, int q_len, int Hq, int Hkv, int head_dim, int num_blocks, int page, int max_blocks,
                             const long long* strides, float scale, void* workspace, void* stream);
 size_t moonmath_gqa_decode_workspace(int B, int q_len, int Hq, int Hkv, int head_dim, int page, int max_blocks,
-                                     const long long* strides);
+                                     int fp8, const long long* strides);
+
+/* How launch_gqa_decode_paged shares a batch of these lengths (host array) out over its
+ * workgroups: 8 ints per segment, {workgroup, request, task of the request, first and
+ * end step (32 tokens each) of it, record that it leaves (-1: none, it is whole),
+ * workgroup from which on the task's records are joined (where the segment ends a task
+ * that was cut, else -1), steps of the task}, tasks in order, the first max_segments of
+ * them. Returns their number; 0: each workgroup takes a task whole. Pure host. */
+int moonmath_gqa_decode_split(int B, const int* lens, int q_len, int Hq, int Hkv, int head_dim, int page,
+                              int max_blocks, int fp8, const long long* strides, int* segments, int max_segments);
 
 /* Rotary positions: pair p of each head of q [B, S, Hq, head_dim] and k [B, S,
  * Hk, head_dim] (Hk 0: q alone) turns by positions[axes[p]][b][s] * turns[p] of a

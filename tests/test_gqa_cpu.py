@@ -103,7 +103,7 @@ def test_refused_distance_of_tokens():
     ({"block_table": z(2, 2, dtype=I32)}, ValueError, "block_table must be \\[B, max_blocks\\]"),
     ({"block_table": z(3, 0, dtype=I32)}, ValueError, "block_table must be \\[B, max_blocks\\]"),
     ({"block_table": z(2, 3, dtype=I32).t()}, ValueError, "last dim must be contiguous"),
-    ({"block_table": z(3, 1, dtype=I32).expand(3, 1 << 27)}, ValueError, "at most 2\\^31 - 64 tokens"),
+    ({"block_table": z(3, 1, dtype=I32).expand(3, 1 << 27)}, ValueError, "at most 2\\^31 - 4096 tokens"),
     ({"q": z(1, 1, 64).expand(3, 65538, 64)}, ValueError, "at most 65536"),
     ({"scale": "x"}, ValueError, "could not convert"),
     ({"out": z(3, 4, 64, dtype=torch.float32)}, ValueError, "out must be bfloat16"),
@@ -296,11 +296,75 @@ def test_workspace():
     """Records depend on the call's shape and not on its lengths; short contexts, empty
     batches and sizes that are refused need none."""
     heads, tokens = ((ctypes.c_longlong * 17)(*[0] * 6, *x) for x in ((1 << 20, 1 << 13, 128), (1 << 16, 128, 1024)))
-    ws = lambda B, D=128, w=128, s=heads: _lib.lib.moonmath_gqa_decode_workspace(B, 1, 32, 8, D, 64, w, s)  # noqa: E731
+    ws = lambda B, D=128, w=128, s=heads: _lib.lib.moonmath_gqa_decode_workspace(B, 1, 32, 8, D, 64, w, 0, s)  # noqa: E731
     assert ws(64, w=2) == 0 and ws(0) == 0 and ws(1, D=96) == 0 and ws(1, s=None) == 0
     for s in (heads, tokens):
         sizes = [ws(B, s=s) for B in (1, 4, 64, 1024)]
         assert 0 < sizes[0] <= sizes[1] <= sizes[2] <= sizes[3] <= sizes[2] + (16 << 10) < 64 << 20
+
+
+HEADS, TOKENS = ((ctypes.c_longlong * 17)(*[0] * 6, *x) for x in ((1 << 20, 1 << 13, 128), (1 << 16, 128, 1024)))
+
+
+def split(lens, q_len, Hq, Hkv, D, page, width, fp8, strides):
+    n = len(lens)
+    arr = (ctypes.c_int * max(n, 1))(*lens)
+    args = (n, arr, q_len, Hq, Hkv, D, page, width, int(fp8), strides)
+    count = _lib.lib.moonmath_gqa_decode_split(*args, None, 0)
+    out = (ctypes.c_int * (8 * max(count, 1)))()
+    assert _lib.lib.moonmath_gqa_decode_split(*args, out, count) == count
+    return [tuple(out[8 * i:8 * i + 8]) for i in range(count)]
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_every_step_is_taken_once(seed):
+    """The shares of random batches: each task's steps once and in order, at most one
+    record of each kind for a workgroup, and the joined workgroups all hold a part; no
+    workgroup has over twice the mean's steps, a task's own cost and a round more."""
+    g = torch.Generator().manual_seed(seed)
+    ri = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=g))  # noqa: E731
+    B = [1, 2, 7, 64, 300, 700][ri(0, 6)]
+    top = [40, 700, 5000, 70000][ri(0, 4)] if B <= 64 else [40, 700, 3000][ri(0, 3)]
+    lens = [0 if ri(0, 9) == 0 else ri(1, top) for _ in range(B)]
+    q_len, (Hq, Hkv) = ri(1, 9), [(8, 1), (4, 2), (16, 16), (32, 8), (48, 1), (24, 3)][ri(0, 6)]
+    D, fp8, strides = [64, 128, 256][ri(0, 3)], bool(ri(0, 2)), [HEADS, TOKENS][ri(0, 2)]
+    width = max(max(lens) // 16 + ri(1, 50), 100)
+    parts = split(lens, q_len, Hq, Hkv, D, 16, width, fp8, strides)
+    if not any(lens):
+        assert parts == []
+        return
+    tasks = {}
+    for p in parts:
+        tasks.setdefault(p[1:3], []).append(p)
+    per = len({t for _, t in tasks})
+    assert len(tasks) == per * sum(n > 0 for n in lens) and per >= 1
+    records, load = set(), {}
+    for (b, _), group in tasks.items():
+        steps = -(-lens[b] // 32)
+        assert group[0][3] == 0 and group[-1][4] == steps and all(p[7] == steps for p in group)
+        assert all(x[4] == y[3] and x[0] + 1 == y[0] for x, y in zip(group, group[1:]))
+        assert all(p[3] < p[4] for p in group)
+        if len(group) == 1:
+            assert group[0][5] == -1 and group[0][6] == -1
+            continue
+        first = group[0][0]
+        assert [p[5] for p in group] == [2 * first + 1] + [2 * p[0] for p in group[1:]]
+        assert [p[6] for p in group] == [-1] * (len(group) - 1) + [first]
+        assert not records & {p[5] for p in group}
+        records |= {p[5] for p in group}
+    for p in parts:
+        load[p[0]] = load.get(p[0], 0) + p[4] - p[3]
+    order = [p[0] for p in parts]
+    assert order == sorted(order) and order[0] >= 0 and order[-1] < 768
+    mean = sum(-(-n // 32) + 12 for n in lens if n) * per / min(768, max(order) + 1)
+    assert max(load.values()) <= 2 * mean + 20
+
+
+def test_split_codes():
+    f, n, st = _lib.lib.moonmath_gqa_decode_split, (ctypes.c_int * 1)(5), HEADS
+    assert f(1, n, 1, 4, 2, 80, 16, 1, 0, st, None, 0) == -2 and f(1, None, 1, 4, 2, 64, 16, 1, 0, st, None, 0) == -6
+    assert f(1, n, 1, 4, 2, 64, 16, 1, 0, None, None, 0) == -6 and f(1, n, 1, 4, 2, 64, 16, 1000, 0, st, None, 4) == -6
+    assert f(0, n, 1, 4, 2, 64, 16, 1000, 0, st, None, 0) == 0 and f(1, n, 1, 4, 2, 64, 16, 1, 0, st, None, 0) == 0
 
 
 def test_native_path_leaves_cpu_calls():
