@@ -74,9 +74,9 @@ constexpr int lead_steps(int D, bool fp8, int rw) { return 4 / rw / 2 + 512 / (f
 // Waves of a workgroup that takes a task whole.
 constexpr int whole_waves(int D, int nt) { return D * nt <= 128 ? 8 : 4; }
 
-// The kernel's shape: NT tiles of 16 rows for each wave, RW row sets; SHARED: of one
-// kv head, so that its rows are read by more than one wave.
-template <int D_, bool FP8_, int NT_, int RW_, bool SHARED_, bool SPLIT_>
+// The kernel's shape: NT tiles of 16 rows for each wave, RW row sets; CACHED: K and V are
+// loaded through the caches, as each is read by several waves, or a line by others.
+template <int D_, bool FP8_, int NT_, int RW_, bool CACHED_, bool SPLIT_>
 struct Shape {
   static constexpr int D = D_, NT = NT_, RW = RW_;
   static constexpr bool FP8 = FP8_, SPLIT = SPLIT_;
@@ -85,7 +85,7 @@ struct Shape {
   static constexpr int kRow = FP8 ? D : 2 * D;          // bytes of a cached row
   static constexpr int kRows = 16 * NT * RW;            // of a task
   static constexpr int kPerCu = SPLIT ? per_cu(D, NT) : 2;
-  static constexpr bool kOnce = !SHARED_ && SPLIT && !(D == 256 && !FP8);  // streamed past the caches
+  static constexpr bool kOnce = !CACHED_ && SPLIT;      // streamed past the caches
   static constexpr int kKLoads = kRow / 64;             // 16-byte loads of K per lane and 16 tokens
   static constexpr int kVWords = kRow / 64;             // dwords of V per lane and token
   static constexpr int kLead = SPLIT ? lead_steps(D, FP8, RW) : 0;
@@ -875,6 +875,7 @@ __global__ __launch_bounds__(kJoinThreads) void gqa_join_kernel(const DecodeArgs
 struct Plan {
   int nt, rw, sets;          // 16-row tiles of a wave, row sets of a task, and of those one kv head's
   int row_blocks, per;       // tasks of a kv head's rows, and of a request
+  int cached;                // whether K and V go through the caches
   int grid, split;           // workgroups; whether they share the steps evenly or take a task each
   long long tasks;
 };
@@ -898,17 +899,26 @@ inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int wi
   p->sets = sets == 1 ? 1 : sets == 2 ? 2 : 4;
   p->rw = p->sets;
   p->split = p->sets > 1 || !short_call(most, (long long)B * Hkv, D, p->nt);
-  // Rows of neighbouring heads: four waves that read them together read whole lines
-  // and neighbouring ones.
+  const long long steps = (most + kStep - 1) / kStep, slots = per_cu(D, p->nt) * kCus;
+  // Rows of neighbouring heads: waves that read them together read whole lines and
+  // neighbouring ones (64 requests of 1K..8K tokens, fp8, 8 heads of 128: 122 us, 136
+  // apart). Their records are as many times larger: only where a run then has steps
+  // enough (one request of 20000, windows of 4: 43 us, 32 apart).
+  const long long blocks = (sets + p->sets - 1) / p->sets;
   if (p->split && by_token)
-    while (p->rw < 4 && 16 * p->nt * p->rw < 64 && Hkv % (p->rw / p->sets * 2) == 0) p->rw *= 2;
+    while (p->rw < 4 && p->nt == 1 && Hkv % (p->rw / p->sets * 2) == 0 &&
+           B * (Hkv / (p->rw / p->sets * 2)) * blocks * steps >= 16 * slots)
+      p->rw *= 2;
+  // Past the caches a row that ends inside a line of 256 bytes costs its neighbour's
+  // reader a second fetch (fp8 rows of 128 apart: 127 us, 140 past them), and so do
+  // bf16 rows of 256 dims, whose halves of lines a wave reads further apart.
+  p->cached = p->sets > 1 || (by_token && p->rw == 1) || (D == 256 && !fp8);
   p->row_blocks = (int)((sets + p->sets - 1) / p->sets);
   const long long per = (long long)(Hkv / (p->rw / p->sets)) * p->row_blocks;
   if (per > 65535) return false;
   p->per = (int)per;
   p->tasks = B * per;
-    const long long steps = (most + 31) / 32, slots = per_cu(D, p->nt) * kCus;
-  const long long places = steps + lead_steps(D, fp8, p->rw);
+    const long long places = steps + lead_steps(D, fp8, p->rw);
   const long long runs = (p->tasks * places * p->rw + 3) / 4;  // of a step for each group of waves
   p->grid = (int)(runs < slots ? runs : slots);
   return p->tasks <= INT_MAX && p->tasks * places < 1LL << 42;  // quotient()'s range
@@ -917,7 +927,7 @@ inline size_t record_bytes(const Plan& p, int D) { return (size_t)2 * p.grid * 1
 // One entry for each task or run, whichever are fewer.
 inline long long join_count(const Plan& p) { return p.tasks < p.grid ? p.tasks : p.grid; }
 
-template <int D, bool FP8, int NT, int RW, bool SHARED>
+template <int D, bool FP8, int NT, int RW, bool CACHED>
 int launch(const DecodeArgs& a, const Plan& p, hipStream_t stream) {
   if (!p.split) {
     if constexpr (RW == 1) {
@@ -925,7 +935,7 @@ int launch(const DecodeArgs& a, const Plan& p, hipStream_t stream) {
       hipLaunchKernelGGL((gqa_decode_kernel<C>), dim3(a.B, p.per), dim3(C::kThreads), 0, stream, a);
     }
   } else {
-    using C = Shape<D, FP8, NT, RW, SHARED, true>;
+    using C = Shape<D, FP8, NT, RW, CACHED, true>;
     hipLaunchKernelGGL((gqa_decode_kernel<C>), dim3(p.grid), dim3(C::kThreads), 0, stream, a);
     // Records of a row: as many as runs share a task, or two ends of a run. A group of
     // lanes takes four at once.
@@ -948,7 +958,8 @@ int launch(const DecodeArgs& a, const Plan& p, hipStream_t stream) {
 template <int D, bool FP8, int NT>
 int with_rw(const DecodeArgs& a, const Plan& p, hipStream_t st) {
   if constexpr (NT > 1 || D == 256)
-    if (p.sets > 1) return p.rw == 2 ? launch<D, FP8, NT, 2, true>(a, p, st) : launch<D, FP8, NT, 4, true>(a, p, st);
+    if (p.rw > 1 && p.cached) return p.rw == 2 ? launch<D, FP8, NT, 2, true>(a, p, st) : launch<D, FP8, NT, 4, true>(a, p, st);
+  if (p.rw == 1 && p.cached) return launch<D, FP8, NT, 1, true>(a, p, st);
   return p.rw == 1   ? launch<D, FP8, NT, 1, false>(a, p, st)
          : p.rw == 2 ? launch<D, FP8, NT, 2, false>(a, p, st)
                      : launch<D, FP8, NT, 4, false>(a, p, st);
