@@ -894,31 +894,35 @@ inline bool token_major(const long long* strides) { return strides[8] > strides[
 inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int width, bool fp8, bool by_token,
                       Plan* p) {
   const long long rows = (long long)(Hq / Hkv) * q_len, most = (long long)page * width;
-  p->nt = rows <= 16 || D == 256 ? 1 : 2;
-  const long long sets = (rows + 16 * p->nt - 1) / (16 * p->nt);
-  p->sets = sets == 1 ? 1 : sets == 2 ? 2 : 4;
+  const long long steps = (most + kStep - 1) / kStep;
+  // Few steps for many rows: 16 rows a task, each reading K and V for itself, rather than
+  // more runs for a task and the records of all its rows (28 requests of 702 tokens, 96
+  // rows: 13 us, 22.5 in tasks of 128 rows; 8 of 2000, 48 rows: 14.8 and 13.9).
+  const bool few = B * Hkv * ((rows + 15) / 16) * steps <= 6LL * per_cu(D, 1) * kCus;
+  p->nt = rows <= 16 || D == 256 || few ? 1 : 2;
+  const long long sets = (rows + 16 * p->nt - 1) / (16 * p->nt), slots = per_cu(D, p->nt) * kCus;
+  p->sets = sets == 1 || few ? 1 : sets == 2 ? 2 : 4;
   p->rw = p->sets;
-  p->split = p->sets > 1 || !short_call(most, (long long)B * Hkv, D, p->nt);
-  const long long steps = (most + kStep - 1) / kStep, slots = per_cu(D, p->nt) * kCus;
+  const long long blocks = (sets + p->sets - 1) / p->sets;
+  p->split = p->sets > 1 || !short_call(most, B * Hkv * blocks, D, p->nt);
   // Rows of neighbouring heads: waves that read them together read whole lines and
   // neighbouring ones (64 requests of 1K..8K tokens, fp8, 8 heads of 128: 122 us, 136
   // apart). Their records are as many times larger: only where a run then has steps
   // enough (one request of 20000, windows of 4: 43 us, 32 apart).
-  const long long blocks = (sets + p->sets - 1) / p->sets;
   if (p->split && by_token)
-    while (p->rw < 4 && p->nt == 1 && Hkv % (p->rw / p->sets * 2) == 0 &&
+    while (p->rw < 4 && p->nt == 1 && blocks == 1 && Hkv % (p->rw / p->sets * 2) == 0 &&
            B * (Hkv / (p->rw / p->sets * 2)) * blocks * steps >= 16 * slots)
       p->rw *= 2;
   // Past the caches a row that ends inside a line of 256 bytes costs its neighbour's
   // reader a second fetch (fp8 rows of 128 apart: 127 us, 140 past them), and so do
   // bf16 rows of 256 dims, whose halves of lines a wave reads further apart.
-  p->cached = p->sets > 1 || (by_token && p->rw == 1) || (D == 256 && !fp8);
-  p->row_blocks = (int)((sets + p->sets - 1) / p->sets);
+  p->cached = sets > 1 || (by_token && p->rw == 1) || (D == 256 && !fp8);
+  p->row_blocks = (int)blocks;
   const long long per = (long long)(Hkv / (p->rw / p->sets)) * p->row_blocks;
   if (per > 65535) return false;
   p->per = (int)per;
   p->tasks = B * per;
-    const long long places = steps + lead_steps(D, fp8, p->rw);
+  const long long places = steps + lead_steps(D, fp8, p->rw);
   const long long runs = (p->tasks * places * p->rw + 3) / 4;  // of a step for each group of waves
   p->grid = (int)(runs < slots ? runs : slots);
   return p->tasks <= INT_MAX && p->tasks * places < 1LL << 42;  // quotient()'s range

@@ -98,6 +98,48 @@ def test_many_rows(D, Hq, Hkv, T):
     run_case([70, 5, 300, 1100], Hq, Hkv, D, T, 64, True, "tokens", seed=Hq)
 
 
+# A table far wider than the requests makes a call be laid out as for long ones: rows of
+# one kv head over several waves, neighbouring heads together, and always shared out.
+WIDE = 4000  # pages of 16
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("Hq,Hkv,T,order", [
+    (4, 2, 1, "heads"), (24, 1, 1, "heads"), (24, 1, 1, "tokens"), (16, 1, 2, "heads"), (48, 1, 1, "heads"),
+    (33, 1, 3, "tokens"), (48, 1, 8, "heads"), (8, 2, 3, "tokens"), (8, 4, 2, "tokens"), (12, 6, 1, "tokens"),
+    (40, 2, 2, "tokens")])
+def test_layouts_of_long_calls(D, fp8, Hq, Hkv, T, order):
+    """1 to 384 query rows for a kv head, one to eight kv heads."""
+    lens = [0, 1, 2, 31, 33, 64, 65, 100, 129, 255, 300, 513, 640, 1000]
+    run_case(lens, Hq, Hkv, D, T, 16, fp8, order, seed=Hq + T, width=WIDE)
+
+
+@pytest.mark.parametrize("T", [1, 2, 5, 8])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 4), (64, 4), (17, 1)])
+def test_windows_in_long_calls(T, Hq, Hkv):
+    """Ends of requests at each place of two steps, where one group of waves has all steps
+    and where several share them."""
+    run_case([1, 2, 7, 8, 9] + list(range(28, 42)) + [63, 64, 65, 70, 96, 97], Hq, Hkv, 64, T, 16, False, "tokens", seed=T,
+             width=WIDE)
+
+
+@pytest.mark.parametrize("bad", [NAN, INF, -INF])
+@pytest.mark.parametrize("Hq,Hkv,width", [(48, 1, WIDE), (8, 4, WIDE), (64, 2, 60), (4, 4, 20)])
+def test_hidden_values_in_every_layout(bad, Hq, Hkv, width):
+    """V of the last three drafts is not finite: each query takes those it sees."""
+    lens = [300, 33, 34, 64]
+    k, v, _, _ = cache(40, Hkv, 16, 64, False, 16, "tokens")
+    table = tables(lens, 16, 40, 16, width)
+    for b, n in enumerate(lens):
+        for t in range(n - 3, n):
+            v[table[b, t // 16], :, t % 16, 5 + t % 3] = bad
+    q = rand_q(4, 4, Hq, 64, 16)
+    out, lse = ma.gqa_decode_paged(q.to(DEV), keep_layout(k), keep_layout(v), torch.tensor(lens, dtype=torch.int32).to(DEV),
+                                   table.to(DEV), return_lse=True)
+    check(out, lse, q, k, v, lens, table)
+
+
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("lens", [[4097], [20000, 3], [65537], [0, 0, 0], [1] * 600, [0] * 299 + [513], [513, 0] * 150])
 def test_lengths(lens, fp8):
