@@ -495,6 +495,38 @@ bool apart(const Tensor& a, const Tensor& b) {
   return end(a) <= reinterpret_cast<uintptr_t>(b.data_ptr()) || end(b) <= reinterpret_cast<uintptr_t>(a.data_ptr());
 }
 
+// Two tensors of one type that are both written, each with its elements apart, share
+// none: they lie apart, or are slices of one tensor (the same steps in the dims that
+// reach past the gap between them, within those all of one before all of the other).
+void share_none(const Tensor& a, const Tensor& b) {
+  if (apart(a, b)) return;
+  const bool swap = reinterpret_cast<uintptr_t>(b.data_ptr()) < reinterpret_cast<uintptr_t>(a.data_ptr());
+  const Tensor &lo = swap ? b : a, &hi = swap ? a : b;
+  const int64_t gap = ((int64_t)(reinterpret_cast<uintptr_t>(hi.data_ptr()) - reinterpret_cast<uintptr_t>(lo.data_ptr()))) /
+                      (int64_t)lo.element_size();
+  std::pair<int64_t, int64_t> outer[4];
+  int n = 0;
+  int64_t first = 1, second = 1;  // what the inner dims of each reach
+  for (int64_t i = 0; i < lo.dim(); ++i) {
+    if (lo.size(i) <= 1 && hi.size(i) <= 1) continue;
+    plain(lo.stride(i) == hi.stride(i));
+    if (lo.stride(i) >= gap) {
+      plain(lo.size(i) == hi.size(i));
+      outer[n++] = {lo.stride(i), lo.size(i)};
+    } else {
+      first += lo.stride(i) * (lo.size(i) - 1);
+      second += hi.stride(i) * (hi.size(i) - 1);
+    }
+  }
+  plain(first <= gap);
+  std::sort(outer, outer + n);
+  int64_t span = gap + second;
+  for (int i = 0; i < n; ++i) {
+    plain(outer[i].first >= span);
+    span += outer[i].first * (outer[i].second - 1);
+  }
+}
+
 bool bool_arg(PyObject* o) {
   plain(PyBool_Check(o));
   return o == Py_True;
@@ -542,6 +574,10 @@ GqaCache gqa_cache(PyObject* k, PyObject* v, PyObject* ks, PyObject* vs, bool wr
       if (fp8) one_place_each(s);
     }
   }
+  if (written) {
+    share_none(c.k, c.v);
+    if (fp8) share_none(c.ks, c.vs);
+  }
   return c;
 }
 
@@ -560,6 +596,7 @@ int64_t gqa_rows(const Tensor& k, const Tensor& v, const Tensor& slots, const Gq
     strides[at++] = t->stride(0);
     strides[at++] = t->stride(1);
   }
+  if (written) share_none(k, v);
   std::copy(c.strides, c.strides + 10, strides + 4);
   return slots.size(0);
 }

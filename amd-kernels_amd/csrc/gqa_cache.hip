@@ -10,7 +10,10 @@
 // HBM bound: 2 bytes of a value on one side, 1 (and 4 / D of the scale) or 2 on the
 // other. A thread holds 16 bytes of the cached row (16 or 8 values) of K and of V, so
 // four or two wide loads are in flight before it waits; a row's D / 16 or D / 8
-// threads lie side by side in one wave, which reduces amax without LDS.
+// threads lie side by side in one wave, which reduces amax without LDS. Written rows go
+// past the caches: 16384 tokens of 8 heads of 128 dims in fp8 17.9 us, 5.5 TB/s (20.2
+// through them). Rows read, and their copies, go through them: 8192 such tokens 11.5
+// us (13.1 to 15 with either past them), 4.3 TB/s with the launch.
 #include <limits.h>
 
 #include "gqa_common.hpp"
@@ -184,7 +187,7 @@ int launch_rows(bool write, const void* k, const void* v, const void* k_cache, c
   const bool fp8 = k_scale != nullptr;
   const int lanes = fp8 ? D / 16 : D / 8;
   const long long grid = (n * heads * lanes + kThreads - 1) / kThreads;
-  if (grid > INT_MAX) return -8;
+  if (grid > UINT_MAX / kThreads) return -8;
   void (*kern)(RowsArgs);
 #define MM_PICK(K)                                                     \
   (fp8 ? (D == 64 ? K<64, true> : D == 128 ? K<128, true> : K<256, true>) \

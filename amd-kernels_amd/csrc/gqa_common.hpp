@@ -25,7 +25,6 @@ constexpr float kFp8Max = 448.f;               // the largest e4m3fn value
 constexpr float kMinScale = 1.17549435e-38f;   // 2^-126: x / scale stays finite for every bf16 row
 
 typedef short s16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 // Four e4m3fn codes -> four bf16 values (exact: e4m3fn is a subset of bf16), in order.
 __device__ __forceinline__ u32x2 fp8x4_to_bf16(uint32_t codes) {

@@ -61,9 +61,9 @@ struct DecodeArgs {
   double per_run;        // 1 / grid
 };
 
-// Workgroups of a CU. One 16-row tile of up to 128 dims fits three waves a SIMD
-// (167 registers of 512); more rows or dims go one a SIMD: two would spill, or write
-// twice the records. 64 requests of 1K..8K tokens, 8 kv heads of 128: two 205 us, three
+// Workgroups of a CU. A 16-row tile of up to 128 dims, or two of 64, fits three waves a
+// SIMD (167 registers of 512); more rows or dims go one a SIMD: two would spill, or
+// write twice the records. 64 requests of 1K..8K tokens, 8 kv heads of 128: two 205 us, three
 // 194; 32 requests of windows of 4, 16 rows a position, 4 kv heads: two 92 us, one 80.
 constexpr int per_cu(int D, int nt) { return D * nt <= 128 ? 3 : 1; }
 
@@ -885,7 +885,8 @@ constexpr int kCus = 256;
 // tasks enough for a quarter of the CUs. One request of 200 tokens (8 kv heads) 7.3 us,
 // shared out 9.0; of 1000 14.1 and 9.5; 64 of up to 500 16.3 and 25, of up to 1000
 // 42.3 and 50; 64 of up to 2000 the same.
-inline bool short_call(long long most, long long tasks, int D, int nt) {
+inline bool short_call(int B, long long most, long long tasks, int D, int nt) {
+  if (B >= 1 << 22) return false;  // a launch has fewer than 2^32 threads along a dimension
   return most <= (tasks >= kCus / 4 ? 4 : 2) * 32 * whole_waves(D, nt);
 }
 
@@ -894,24 +895,25 @@ inline bool token_major(const long long* strides) { return strides[8] > strides[
 inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int width, bool fp8, bool by_token,
                       Plan* p) {
   const long long rows = (long long)(Hq / Hkv) * q_len, most = (long long)page * width;
-  const long long steps = (most + kStep - 1) / kStep;
+  const long long steps = (most + kStep - 1) / kStep, all = (long long)B * Hkv;
+  if (all * ((rows + 15) / 16) > INT_MAX) return false;
   // Few steps for many rows: 16 rows a task, each reading K and V for itself, rather than
   // more runs for a task and the records of all its rows (28 requests of 702 tokens, 96
   // rows: 13 us, 22.5 in tasks of 128 rows; 8 of 2000, 48 rows: 14.8 and 13.9).
-  const bool few = B * Hkv * ((rows + 15) / 16) * steps <= 6LL * per_cu(D, 1) * kCus;
+  const bool few = all * ((rows + 15) / 16) * steps <= 6LL * per_cu(D, 1) * kCus;
   p->nt = rows <= 16 || D == 256 || few ? 1 : 2;
   const long long sets = (rows + 16 * p->nt - 1) / (16 * p->nt), slots = per_cu(D, p->nt) * kCus;
   p->sets = sets == 1 || few ? 1 : sets == 2 ? 2 : 4;
   p->rw = p->sets;
   const long long blocks = (sets + p->sets - 1) / p->sets;
-  p->split = p->sets > 1 || !short_call(most, B * Hkv * blocks, D, p->nt);
+  p->split = p->sets > 1 || !short_call(B, most, all * blocks, D, p->nt);
   // Rows of neighbouring heads: waves that read them together read whole lines and
   // neighbouring ones (64 requests of 1K..8K tokens, fp8, 8 heads of 128: 122 us, 136
   // apart). Their records are as many times larger: only where a run then has steps
   // enough (one request of 20000, windows of 4: 43 us, 32 apart).
   if (p->split && by_token)
     while (p->rw < 4 && p->nt == 1 && blocks == 1 && Hkv % (p->rw / p->sets * 2) == 0 &&
-           B * (Hkv / (p->rw / p->sets * 2)) * blocks * steps >= 16 * slots)
+           all / (p->rw / p->sets * 2) * steps >= 16 * slots)
       p->rw *= 2;
   // Past the caches a row that ends inside a line of 256 bytes costs its neighbour's
   // reader a second fetch (fp8 rows of 128 apart: 127 us, 140 past them), and so do
@@ -925,7 +927,7 @@ inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int wi
   const long long places = steps + lead_steps(D, fp8, p->rw);
   const long long runs = (p->tasks * places * p->rw + 3) / 4;  // of a step for each group of waves
   p->grid = (int)(runs < slots ? runs : slots);
-  return p->tasks <= INT_MAX && p->tasks * places < 1LL << 42;  // quotient()'s range
+  return p->tasks * places < 1LL << 42;  // quotient()'s range
 }
 inline size_t record_bytes(const Plan& p, int D) { return (size_t)2 * p.grid * 16 * p.nt * p.rw * (D + 2) * 4; }
 // One entry for each task or run, whichever are fewer.
@@ -958,15 +960,26 @@ int launch(const DecodeArgs& a, const Plan& p, hipStream_t stream) {
   return e == hipSuccess ? 0 : (int)e;
 }
 
-// NT 1 of up to 128 dims is one row set.
+// The shapes that plan_call() chooses: several row sets of one kv head go through the
+// caches, and so does bf16 of 256 dims; heads are grouped in single tiles only.
 template <int D, bool FP8, int NT>
 int with_rw(const DecodeArgs& a, const Plan& p, hipStream_t st) {
-  if constexpr (NT > 1 || D == 256)
-    if (p.rw > 1 && p.cached) return p.rw == 2 ? launch<D, FP8, NT, 2, true>(a, p, st) : launch<D, FP8, NT, 4, true>(a, p, st);
-  if (p.rw == 1 && p.cached) return launch<D, FP8, NT, 1, true>(a, p, st);
-  return p.rw == 1   ? launch<D, FP8, NT, 1, false>(a, p, st)
-         : p.rw == 2 ? launch<D, FP8, NT, 2, false>(a, p, st)
-                     : launch<D, FP8, NT, 4, false>(a, p, st);
+  constexpr bool kCachedOnly = D == 256 && !FP8;
+  if (p.cached) {
+    if constexpr (NT > 1 || D == 256) {
+      if (p.rw == 2) return launch<D, FP8, NT, 2, true>(a, p, st);
+      if (p.rw == 4) return launch<D, FP8, NT, 4, true>(a, p, st);
+    }
+    return launch<D, FP8, NT, 1, true>(a, p, st);
+  }
+  if constexpr (!kCachedOnly) {
+    if constexpr (NT == 1) {
+      if (p.rw == 2) return launch<D, FP8, NT, 2, false>(a, p, st);
+      if (p.rw == 4) return launch<D, FP8, NT, 4, false>(a, p, st);
+    }
+    return launch<D, FP8, NT, 1, false>(a, p, st);
+  }
+  return -8;
 }
 template <bool FP8>
 int dispatch(const DecodeArgs& a, const Plan& p, int D, hipStream_t st) {

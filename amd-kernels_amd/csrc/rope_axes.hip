@@ -169,7 +169,7 @@ int launch_rope_axes(const void* q, const void* k, void* q_out, void* k_out, con
   // A token for each workgroup, or four where its heads would leave half the threads idle.
   const int all = Hq + Hk, tokens = (long long)all * (head_dim / 16) > kThreads / 2 ? 1 : 4;
   const long long grid = (a.tokens + tokens - 1) / tokens;
-  if (grid > INT_MAX) return -8;
+  if (grid > UINT_MAX / kThreads) return -8;
   // Few tokens: the heads are shared out over more workgroups, up to two for each CU.
   const int once = heads_at_once(head_dim, tokens);
   const long long visits = (all + (long long)once - 1) / once;

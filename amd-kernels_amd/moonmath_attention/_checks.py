@@ -50,3 +50,25 @@ def extent(t):
 def apart(a, b):
     (a0, a1), (b0, b1) = extent(a), extent(b)
     return a1 <= b0 or b1 <= a0
+
+
+def share_none(a, b):
+    """Whether two tensors of one type that are both written, each with its elements
+    apart, are seen to share none: they lie apart, or are slices of one tensor (the
+    same steps in the dims that reach past the gap between them, and within those
+    steps all of one before all of the other)."""
+    if apart(a, b):
+        return True
+    lo, hi = (a, b) if a.data_ptr() < b.data_ptr() else (b, a)
+    gap = (hi.data_ptr() - lo.data_ptr()) // lo.element_size()
+    dims = [i for i in range(a.dim()) if lo.shape[i] > 1 or hi.shape[i] > 1]
+    outer = [i for i in dims if lo.stride(i) >= gap]
+    if any(lo.stride(i) != hi.stride(i) for i in dims) or any(lo.shape[i] != hi.shape[i] for i in outer):
+        return False
+    reach = [sum(t.stride(i) * (t.shape[i] - 1) for i in dims if i not in outer) + 1 for t in (lo, hi)]
+    span = gap + reach[1]
+    for s, n in sorted((lo.stride(i), lo.shape[i]) for i in outer):
+        if s < span:
+            return False
+        span += s * (n - 1)
+    return reach[0] <= gap

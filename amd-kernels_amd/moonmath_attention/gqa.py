@@ -70,6 +70,8 @@ def _check_cache(k_cache, v_cache, k_scale, v_scale, who, written):
             ck.rows(t, name, who)
             if written:
                 ck.one_place_each(t, name, who)
+    if written and not (ck.share_none(k_cache, v_cache) and (not fp8 or ck.share_none(k_scale, v_scale))):
+        raise ValueError(f"{who}: the K and V caches must not share memory")
     return nb, heads, page, D, fp8
 
 
@@ -104,6 +106,8 @@ def _check_rows(k, v, slots, heads, D, who, written):
     N = k.shape[0]
     if v.shape[0] != N:
         raise ValueError(f"{who}: k and v must hold the same number of tokens")
+    if written and not ck.share_none(k, v):
+        raise ValueError(f"{who}: k and v are written, and must not share memory")
     if slots.dim() != 1 or slots.shape[0] != N or not slots.is_contiguous():
         raise ValueError(f"{who}: slots must be contiguous with one entry per token ({N}), got {list(slots.shape)}")
     return N
@@ -191,8 +195,10 @@ def gqa_decode_paged(q, k_cache, v_cache, seq_lens, block_table, *, scale=None, 
     softmax's sum, by which outputs over parts of a context join. A query that sees no
     token gives zeros and -inf. Table entries past a request's length are not used,
     and what cache rows past it hold reaches no output; lengths are clamped to
-    [0, max_blocks * page], page ids to the cache. Calls share nothing: each takes
-    its own workspace from torch's allocator.
+    [0, max_blocks * page], page ids to the cache. Sums of weighted V are held in
+    float32 before they are divided by the weights' sum: |V| times the number of
+    tokens has to stay below 3.4e38. Calls share nothing: each takes its own
+    workspace from torch's allocator.
     """
     res = _lib.calls.gqa_decode(q, k_cache, v_cache, seq_lens, block_table, scale, k_scale, v_scale, out, return_lse)
     if res is not None:

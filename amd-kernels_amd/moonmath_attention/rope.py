@@ -110,7 +110,7 @@ class AxialRope:
             ck.rows(t, name, who)
             if inplace:
                 ck.one_place_each(t, name, who)
-        if inplace and k is not None and not _can_share(q, k):
+        if inplace and k is not None and not ck.share_none(q, k):
             raise ValueError(f"{who}: q and k must not share elements when they are written in place")
         B, S = q.shape[0], q.shape[sax]
         if not isinstance(positions, torch.Tensor) or positions.dtype != torch.int32:
@@ -133,23 +133,3 @@ class AxialRope:
             if rc != 0:
                 raise RuntimeError(f"launch_rope_axes returned error code {rc}")
         return outs[0], outs[1]
-
-
-def _can_share(q, k):
-    """Whether two tensors that are both written share no element: apart, or slices of
-    one fused tensor (equal strides, the second's rows beside the first's)."""
-    if ck.apart(q, k):
-        return True
-    # Heads of one fused row: equal steps from token to token, and all heads of one
-    # lie before those of the other within that step.
-    es = q.element_size()
-    lo, hi = (q, k) if q.data_ptr() < k.data_ptr() else (k, q)
-    gap = (hi.data_ptr() - lo.data_ptr()) // es
-    dims = [i for i in range(4) if lo.shape[i] > 1 or hi.shape[i] > 1]
-    inner = [i for i in dims if lo.stride(i) < gap]
-    outer = [i for i in dims if lo.stride(i) >= gap]
-    if any(lo.stride(i) != hi.stride(i) for i in dims) or any(lo.shape[i] != hi.shape[i] for i in outer):
-        return False
-    reach = [sum(t.stride(i) * (t.shape[i] - 1) for i in inner) + 1 for t in (lo, hi)]
-    step = min((lo.stride(i) for i in outer), default=None)
-    return reach[0] <= gap and (step is None or gap + reach[1] <= step)

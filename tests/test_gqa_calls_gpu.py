@@ -91,6 +91,27 @@ def test_plain_calls_are_taken():
     torch.cuda.synchronize()
 
 
+def test_caches_in_one_tensor_are_taken():
+    c = _lib.calls
+    n = torch.ones(1, dtype=torch.int32, device=DEV)
+    x = torch.ones(1, 2, 64, dtype=torch.bfloat16, device=DEV)
+    one = torch.zeros(4, 2, 2, 16, 64, dtype=torch.bfloat16, device=DEV)
+    pairs = [(one[:, 0], one[:, 1]), (one[:, :, 1], one[:, :, 0]), (one.view(2, 4, 2, 16, 64)[0], one.view(2, 4, 2, 16, 64)[1]),
+             tuple(one.view(4, 16, 2, 2, 64).select(3, i).transpose(1, 2) for i in (0, 1)),
+             tuple(one.view(4, 2, 16, 128)[..., 64 * i:64 * i + 64] for i in (0, 1))]
+    for k, v in pairs:
+        one.zero_()
+        assert c.gqa_write(x, 2 * x, k, v, n, None, None) is True
+        assert k.float().sum() == 128 and v.float().sum() == 256
+        assert c.gqa_write(x, x, k, k, n, None, None) is None
+        assert c.gqa_write(x, x, k[1:], k[:-1], n, None, None) is None
+    k, v = pairs[0]
+    out = torch.empty(1, 2, 2, 64, dtype=torch.bfloat16, device=DEV)
+    assert c.gqa_read(k, v, n, None, None, out[:, 0], out[:, 1]) is not None
+    assert c.gqa_read(k, v, n, None, None, out[:, 0], out[:, 0]) is None
+    torch.cuda.synchronize()
+
+
 def test_refusals_on_the_gpu():
     k, v, _, _ = (None if t is None else t.to(DEV) for t in cache(4, 2, 16, 64, False, 3))
     q = torch.zeros(1, 4, 64, dtype=torch.bfloat16, device=DEV)

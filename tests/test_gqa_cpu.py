@@ -229,8 +229,6 @@ def _shares(q, k):
 
 def test_views_that_are_written_together():
     """Whatever views pass for sharing nothing do share nothing."""
-    from moonmath_attention.rope import _can_share
-
     g = torch.Generator().manual_seed(1)
     ri = lambda lo, hi: int(torch.randint(lo, hi, (1,), generator=g))  # noqa: E731
     base, passed = torch.zeros(4000, dtype=BF), 0
@@ -241,10 +239,43 @@ def test_views_that_are_written_together():
             shape = (ri(1, 3), ri(1, 5), ri(1, H + 1), 8)
             views.append(base.as_strided(shape, (rowlen * 5, rowlen, 8, 1) if ri(0, 4) else (8 * ri(0, 60), 8 * ri(0, 9), 8, 1),
                                          8 * ri(0, 12)))
-        if _can_share(*views):
+        if _checks.share_none(*views):
             passed += 1
             assert not _shares(*views), [(v.shape, v.stride(), v.storage_offset()) for v in views]
     assert passed > 100
+    # Steps that do not nest: the second view's rows lie between the first's, and on some.
+    lo, hi = (base.as_strided((2, 2, 1, 8), (120, 80, 8, 1), at) for at in (0, 40))
+    _checks.one_place_each(lo, "lo", "who")
+    assert _shares(lo, hi) and not _checks.share_none(lo, hi)
+
+
+@pytest.mark.parametrize("shape,dim,order", [((2, 6, 2, 16, 64), 0, None), ((6, 2, 2, 16, 64), 1, None),
+                                             ((6, 16, 2, 2, 64), 2, (0, 2, 1, 3)), ((6, 16, 2, 2, 64), 3, (0, 2, 1, 3)),
+                                             ((6, 2, 16, 128), None, None)])
+def test_caches_in_one_tensor(shape, dim, order):
+    """K and V as slices of one tensor are written; one over the other is refused."""
+    x = z(*shape)
+    k, v = (x[..., :64], x[..., 64:]) if dim is None else (x.select(dim, 0), x.select(dim, 1))
+    if order:
+        k, v = k.permute(order), v.permute(order)
+    with pytest.raises(ValueError, match="on a CUDA/HIP device"):
+        write(k_cache=k, v_cache=v)
+    for a, b in ((k, k), (v, v), (k[1:], k[:-1])):
+        with pytest.raises(ValueError, match="must not share memory"):
+            write(k_cache=a, v_cache=b)
+
+
+def test_results_in_one_place():
+    x = z(5, 2, 2, 64)
+    with pytest.raises(ValueError, match="on a CUDA/HIP device"):
+        read(k=x[:, 0], v=x[:, 1])
+    with pytest.raises(ValueError, match="must not share memory"):
+        read(k=x[:, 0], v=x[:, 0])
+    c = good(True)
+    with pytest.raises(ValueError, match="must not share memory"):
+        write(**{**c, "v_scale": c["k_scale"]})
+    with pytest.raises(ValueError, match="on a CUDA/HIP device"):  # read alone, they may be one
+        decode(**{**c, "v_cache": c["k_cache"], "v_scale": c["k_scale"]})
 
 
 def test_memory_checks_of_views():
@@ -279,17 +310,21 @@ def test_launcher_codes():
     far[8] = (1 << 26) + 1
     assert dec(s=far) == -9
     assert dec(B=0) == 0
+    # Sizes that no launch takes, past 31 bits in products of two or three of them.
+    assert dec(B=1 << 30, Hq=16, Hkv=8, ws=p) == -8 and dec(B=1 << 16, Hq=1 << 16, Hkv=1 << 16, w=1000, ws=p) == -8
+    assert lib.moonmath_gqa_decode_workspace(1 << 30, 1, 16, 8, 64, 16, 1000, 0, st) == 0
     for fn, order in ((lib.launch_gqa_kv_write, lambda k, ks: (k, p, p, p, ks, n, p)),
                       (lib.launch_gqa_kv_read, lambda k, ks: (p, p, ks, n, p, k, p))):
         run = lambda N=1, H=1, D=64, nb=1, page=16, k=p, ks=n, s=st: fn(*order(k, ks), N, H, D, nb, page, s, n)  # noqa: E731
         assert run(D=32) == -2 and run(H=0) == -3 and run(N=-1) == -4 and run(page=20) == -5 and run(nb=-1) == -11
         assert run(nb=1 << 28) == -11 and run(k=n) == -6 and run(ks=p) == -6 and run(s=None) == -6
-        assert run(N=1 << 40) == -8 and run(N=0) == 0
+        assert run(N=1 << 40) == -8 and run(N=1 << 31) == -8 and run(N=0) == 0
     rope = lambda B=1, S=1, Hq=1, Hk=0, D=64, P=8, A=1, q=p, s=st: (  # noqa: E731
         lib.launch_rope_axes(q, n, p, n, p, p, p, B, S, Hq, Hk, D, P, A, 0, 0, s, n))
     assert rope(D=32) == -2 and rope(Hq=0) == -3 and rope(Hk=-1) == -3 and rope(B=-1) == -4 and rope(S=-1) == -4
     assert rope(P=4) == -5 and rope(P=12) == -5 and rope(P=40) == -5 and rope(A=0) == -5
     assert rope(q=n) == -6 and rope(Hk=1) == -6 and rope(s=None) == -6 and rope(S=0) == 0 and rope(B=0) == 0
+    assert rope(B=1 << 10, S=1 << 20) == -8
 
 
 def test_workspace():

@@ -124,6 +124,20 @@ def test_windows_in_long_calls(T, Hq, Hkv):
              width=WIDE)
 
 
+@pytest.mark.parametrize("D,B,width,fp8", [(64, 100, 60, False), (64, 100, 60, True), (128, 150, 32, False),
+                                           (128, 150, 32, True)])
+def test_many_short_requests_of_many_rows(D, B, width, fp8):
+    """24 rows for each workgroup that takes a request whole."""
+    run_case([(37 * i) % (16 * width - 1) if i % 9 == 0 else i % 50 for i in range(B)], 24, 1, D, 1, 16, fp8, "heads", seed=B,
+             width=width)
+
+
+def test_a_large_batch():
+    """More requests than threads look for a run's first one; most of them empty in places."""
+    run_case([(7 * i) % 70 if i % 600 > 40 or i % 7 == 0 else 0 for i in range(1500)], 2, 2, 64, 2, 16, False, "heads",
+             width=200)
+
+
 @pytest.mark.parametrize("bad", [NAN, INF, -INF])
 @pytest.mark.parametrize("Hq,Hkv,width", [(48, 1, WIDE), (8, 4, WIDE), (64, 2, 60), (4, 4, 20)])
 def test_hidden_values_in_every_layout(bad, Hq, Hkv, width):
