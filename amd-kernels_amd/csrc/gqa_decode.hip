@@ -74,8 +74,8 @@ constexpr int lead_steps(int D, bool fp8, int rw) { return 4 / rw / 2 + 512 / (f
 // Waves of a workgroup that takes a task whole.
 constexpr int whole_waves(int D, int nt) { return D * nt <= 128 ? 8 : 4; }
 
-// The kernel's shape: NT tiles of 16 rows for each wave, RW row sets; CACHED: K and V are
-// loaded through the caches, as each is read by several waves, or a line by others.
+// The kernel's shape: NT tiles of 16 rows for each wave, RW row sets; CACHED: V is loaded
+// through the caches, as several waves read it.
 template <int D_, bool FP8_, int NT_, int RW_, bool CACHED_, bool SPLIT_>
 struct Shape {
   static constexpr int D = D_, NT = NT_, RW = RW_;
@@ -85,7 +85,7 @@ struct Shape {
   static constexpr int kRow = FP8 ? D : 2 * D;          // bytes of a cached row
   static constexpr int kRows = 16 * NT * RW;            // of a task
   static constexpr int kPerCu = SPLIT ? per_cu(D, NT) : 2;
-  static constexpr bool kOnce = !CACHED_ && SPLIT;      // streamed past the caches
+  static constexpr bool kOnce = !CACHED_ && SPLIT;      // V is streamed past the caches
   static constexpr int kKLoads = kRow / 64;             // 16-byte loads of K per lane and 16 tokens
   static constexpr int kVWords = kRow / 64;             // dwords of V per lane and token
   static constexpr int kLead = SPLIT ? lead_steps(D, FP8, RW) : 0;
@@ -144,8 +144,10 @@ __device__ __forceinline__ Pages<C> step_pages(const DecodeArgs& a, ConstInts ro
   return p;
 }
 
-// Streamed once: nothing of it is read again by this launch but the other half of a
-// line by the next load.
+// V's rows are read whole by one load each, and once. K goes through the caches: a load
+// takes 64 bytes of each of 16 rows, the next one the other half of their lines (64
+// requests of 1K..8K tokens, 8 kv heads of 128, bf16: both through the caches 209 us,
+// both past them 192, K past them 206, V alone 181; fp8: 118, 111, 121 and 105).
 template <class T, bool ONCE>
 __device__ __forceinline__ T stream(const char* p) {
   if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
@@ -153,16 +155,16 @@ __device__ __forceinline__ T stream(const char* p) {
 }
 
 template <class C>
-__device__ __forceinline__ void load_k(const DecodeArgs& a, Step<C>& s, const Pages<C>& pg, int tok, int head,
-                                       int lane) {
+__device__ __forceinline__ void load_k(const DecodeArgs& a, Step<C>& s, const Pages<C>& pg, int tok, int head, int lane,
+                                       uint32_t mask = ~0u) {
   constexpr int kElem = C::FP8 ? 1 : 2;
-  const uint32_t off = (uint32_t)(lane & 15) * (uint32_t)(a.k.row_s * kElem) + 16u * (lane >> 4);
+  const uint32_t off = ((uint32_t)(lane & 15) * (uint32_t)(a.k.row_s * kElem) + 16u * (lane >> 4)) & mask;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = (tok + 16 * i) & ((1 << a.page_shift) - 1);
     const char* kb = a.k.base + (pg.id[i] * a.k.block_s + head * a.k.head_s + row * a.k.row_s) * kElem;
 #pragma unroll
-    for (int c = 0; c < C::kKLoads; ++c) s.k[i][c] = stream<u32x4, C::kOnce>(kb + off + 64 * c);
+    for (int c = 0; c < C::kKLoads; ++c) s.k[i][c] = *reinterpret_cast<const u32x4*>(kb + off + 64 * c);
     if constexpr (C::FP8)
       s.ks[i] = *reinterpret_cast<const f32x4*>(a.k.scale + pg.id[i] * a.k.sblock_s + head * a.k.shead_s + row +
                                                 4 * (lane >> 4));
@@ -170,10 +172,10 @@ __device__ __forceinline__ void load_k(const DecodeArgs& a, Step<C>& s, const Pa
 }
 
 template <class C>
-__device__ __forceinline__ void load_v(const DecodeArgs& a, Step<C>& s, const Pages<C>& pg, int tok, int head,
-                                       int lane) {
+__device__ __forceinline__ void load_v(const DecodeArgs& a, Step<C>& s, const Pages<C>& pg, int tok, int head, int lane,
+                                       uint32_t mask = ~0u) {
   constexpr int kElem = C::FP8 ? 1 : 2;
-  const uint32_t off = 4u * (lane >> 4) * (uint32_t)(a.v.row_s * kElem) + (uint32_t)(C::kVWords * 4 * (lane & 15));
+  const uint32_t off = (4u * (lane >> 4) * (uint32_t)(a.v.row_s * kElem) + (uint32_t)(C::kVWords * 4 * (lane & 15))) & mask;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int row = (tok + 16 * i) & ((1 << a.page_shift) - 1);
@@ -289,7 +291,7 @@ __device__ __forceinline__ void add_pv(Rows<C>& w, const Step<C>& s, const bf16x
 // about a step (16 KB) is in flight for each wave at any time.
 template <class C, bool TAIL>
 __device__ __forceinline__ void compute_step(const DecodeArgs& a, Rows<C>& w, Step<C>& s, int tok, int len,
-                                             const Pages<C>& pg, int next, int head, int lane) {
+                                             const Pages<C>& pg, int next, uint32_t mask, int head, int lane) {
   const int tok0 = tok + 4 * (lane >> 4);  // this lane's tokens: tok0 + 16 i + r
   f32x4 sc[C::NT][2];
 #pragma unroll
@@ -326,7 +328,7 @@ __device__ __forceinline__ void compute_step(const DecodeArgs& a, Rows<C>& w, St
   for (int i = 0; i < 2; ++i) ks[i] = s.ks[i];
   if constexpr (!TAIL) {
     sched_fence();
-    load_k<C>(a, s, pg, next, head, lane);
+    load_k<C>(a, s, pg, next, head, lane, mask);
     sched_fence();
   }
 #pragma unroll
@@ -389,7 +391,7 @@ __device__ __forceinline__ void compute_step(const DecodeArgs& a, Rows<C>& w, St
     for (int t = apiece ? 0 : a.q_len - 1; t < a.q_len; ++t)
       add_pv<C, true>(w, s, hi, lo, tok0, len - a.q_len + t + 1, apiece ? t : -1);
   }
-  if constexpr (!TAIL) load_v<C>(a, s, pg, next, head, lane);
+  if constexpr (!TAIL) load_v<C>(a, s, pg, next, head, lane, mask);
 }
 
 // x / d of whole numbers below 2^52 (inv: 1 / d, rounded): the rounded product is at
@@ -658,8 +660,9 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
 
     // A wave's steps are every kGroups-th one. Those from s_full on hold tokens that
     // some position does not see: a step's worth and q_len - 1, in two steps at most.
-    // Loads past the last step repeat it: one under a branch would make the compiler
-    // wait for all of them.
+    // Loads past the last step read its first row of each 16 or 4 over again (mask 0):
+    // a load under a branch would make the compiler wait for all of them, and the whole
+    // step again was 4% of the bytes read.
     {
       const ConstInts table = (ConstInts)(uintptr_t)(a.table + (long long)x.b * a.table_s);
       int head, row0;
@@ -675,12 +678,12 @@ __global__ __launch_bounds__(C::kThreads, C::kPerCu) void gqa_decode_kernel(cons
         for (; st <= s_last && st < s_full; st += C::kGroups) {
           const int after = min(next + C::kGroups, s_last);
           const Pages<C> pa = step_pages<C>(a, table, after * kStep);
-          compute_step<C, false>(a, w, s, st * kStep, x.len, pg, next * kStep, head, lane);
+          compute_step<C, false>(a, w, s, st * kStep, x.len, pg, next * kStep, st < s_last ? ~0u : 0u, head, lane);
           pg = pa;
           next = after;
         }
         while (st <= s_last) {
-          compute_step<C, true>(a, w, s, st * kStep, x.len, pg, 0, head, lane);
+          compute_step<C, true>(a, w, s, st * kStep, x.len, pg, 0, 0u, head, lane);
           st += C::kGroups;
           if (C::kGroups > 1 || st > s_last) break;  // a wave of several has one such step
           pg = step_pages<C>(a, table, st * kStep);
@@ -875,18 +878,20 @@ __global__ __launch_bounds__(kJoinThreads) void gqa_join_kernel(const DecodeArgs
 struct Plan {
   int nt, rw, sets;          // 16-row tiles of a wave, row sets of a task, and of those one kv head's
   int row_blocks, per;       // tasks of a kv head's rows, and of a request
-  int cached;                // whether K and V go through the caches
+  int cached;                // whether V goes through the caches
   int grid, split;           // workgroups; whether they share the steps evenly or take a task each
   long long tasks;
 };
 constexpr int kCus = 256;
 // Whether a workgroup takes each task whole, without the plan's reads and the second
 // launch: where the longest request is two steps of each wave, or four where there are
-// tasks enough for a quarter of the CUs. One request of 200 tokens (8 kv heads) 7.3 us,
-// shared out 9.0; of 1000 14.1 and 9.5; 64 of up to 500 16.3 and 25, of up to 1000
-// 42.3 and 50; 64 of up to 2000 the same.
-inline bool short_call(int B, long long most, long long tasks, int D, int nt) {
-  if (B >= 1 << 22) return false;  // a launch has fewer than 2^32 threads along a dimension
+// tasks enough for a quarter of the CUs; but not where there are more tasks than two for
+// each CU (of rows of 256 bytes; more of shorter ones), as most waves of a short one have
+// nothing to do. One request of 200 tokens (8 kv heads of 128, bf16) 6.7 us, shared out
+// 9.0; of 1000 14.1 and 9.5; 64 of up to 500 16.3 and 25; 128 of up to 500 39 and 35 (fp8
+// 21 and 27), 256 of up to 60 36 and 25 (fp8 22 and 23).
+inline bool short_call(long long most, long long tasks, int D, int nt, bool fp8) {
+  if (tasks * (fp8 ? D : 2 * D) > 2 * kCus * 256) return false;
   return most <= (tasks >= kCus / 4 ? 4 : 2) * 32 * whole_waves(D, nt);
 }
 
@@ -906,7 +911,7 @@ inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int wi
   p->sets = sets == 1 || few ? 1 : sets == 2 ? 2 : 4;
   p->rw = p->sets;
   const long long blocks = (sets + p->sets - 1) / p->sets;
-  p->split = p->sets > 1 || !short_call(B, most, all * blocks, D, p->nt);
+  p->split = p->sets > 1 || !short_call(most, all * blocks, D, p->nt, fp8);
   // Rows of neighbouring heads: waves that read them together read whole lines and
   // neighbouring ones (64 requests of 1K..8K tokens, fp8, 8 heads of 128: 122 us, 136
   // apart). Their records are as many times larger: only where a run then has steps
@@ -915,10 +920,7 @@ inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int wi
     while (p->rw < 4 && p->nt == 1 && blocks == 1 && Hkv % (p->rw / p->sets * 2) == 0 &&
            all / (p->rw / p->sets * 2) * steps >= 16 * slots)
       p->rw *= 2;
-  // Past the caches a row that ends inside a line of 256 bytes costs its neighbour's
-  // reader a second fetch (fp8 rows of 128 apart: 127 us, 140 past them), and so do
-  // bf16 rows of 256 dims, whose halves of lines a wave reads further apart.
-  p->cached = sets > 1 || (by_token && p->rw == 1) || (D == 256 && !fp8);
+  p->cached = p->sets > 1;
   p->row_blocks = (int)blocks;
   const long long per = (long long)(Hkv / (p->rw / p->sets)) * p->row_blocks;
   if (per > 65535) return false;
@@ -960,25 +962,15 @@ int launch(const DecodeArgs& a, const Plan& p, hipStream_t stream) {
   return e == hipSuccess ? 0 : (int)e;
 }
 
-// The shapes that plan_call() chooses: several row sets of one kv head go through the
-// caches, and so does bf16 of 256 dims; heads are grouped in single tiles only.
+// The shapes that plan_call() chooses: row sets of one kv head are of two tiles, or of 256
+// dims, and heads are grouped in single tiles.
 template <int D, bool FP8, int NT>
 int with_rw(const DecodeArgs& a, const Plan& p, hipStream_t st) {
-  constexpr bool kCachedOnly = D == 256 && !FP8;
-  if (p.cached) {
-    if constexpr (NT > 1 || D == 256) {
-      if (p.rw == 2) return launch<D, FP8, NT, 2, true>(a, p, st);
-      if (p.rw == 4) return launch<D, FP8, NT, 4, true>(a, p, st);
-    }
-    return launch<D, FP8, NT, 1, true>(a, p, st);
-  }
-  if constexpr (!kCachedOnly) {
-    if constexpr (NT == 1) {
-      if (p.rw == 2) return launch<D, FP8, NT, 2, false>(a, p, st);
-      if (p.rw == 4) return launch<D, FP8, NT, 4, false>(a, p, st);
-    }
-    return launch<D, FP8, NT, 1, false>(a, p, st);
-  }
+  if (p.rw == 1) return launch<D, FP8, NT, 1, false>(a, p, st);
+  if constexpr (NT > 1 || D == 256)
+    if (p.cached) return p.rw == 2 ? launch<D, FP8, NT, 2, true>(a, p, st) : launch<D, FP8, NT, 4, true>(a, p, st);
+  if constexpr (NT == 1)
+    if (!p.cached) return p.rw == 2 ? launch<D, FP8, NT, 2, false>(a, p, st) : launch<D, FP8, NT, 4, false>(a, p, st);
   return -8;
 }
 template <bool FP8>
