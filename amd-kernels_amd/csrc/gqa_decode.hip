@@ -61,14 +61,16 @@ struct DecodeArgs {
   double per_run;        // 1 / grid
 };
 
-// Workgroups of a CU. A 16-row tile of up to 128 dims, or two of 64, fits three waves a
-// SIMD (167 registers of 512); more rows or dims go one a SIMD: two would spill, or
-// write twice the records. 64 requests of 1K..8K tokens, 8 kv heads of 128: two 205 us, three
-// 194; 32 requests of windows of 4, 16 rows a position, 4 kv heads: two 92 us, one 80.
-constexpr int per_cu(int D, int nt) { return D * nt <= 128 ? 3 : 1; }
+// Workgroups of a CU: two where a 16-row tile of up to 128 dims, or two of 64, fits two
+// waves a SIMD with room, else one. Three leave more records and more starts: one request
+// of 65537 tokens fp8 30.4 us, 31.5; 64 of 1K..8K, 8 kv heads of 64, fp8, token-major
+// 76, 84; 8 of 128, bf16 195, 199. Two of a 32-row tile of 128 dims: 32 requests of
+// windows of 4, 16 rows a position, 4 kv heads 86 us, one 79.
+constexpr int per_cu(int D, int nt) { return D * nt <= 128 ? 2 : 1; }
 
 // What a task's start and end cost a workgroup, as steps: about 4 us, in which one of
-// three on a CU streams 32 KB, and half a step of each group of waves that has none.
+// two on a CU streams some 48 KB (half and three times as much counted for it measured
+// alike), and half a step of each group of waves that has none.
 constexpr int lead_steps(int D, bool fp8, int rw) { return 4 / rw / 2 + 512 / (fp8 ? D : 2 * D); }
 
 // Waves of a workgroup that takes a task whole.
@@ -886,12 +888,12 @@ constexpr int kCus = 256;
 // Whether a workgroup takes each task whole, without the plan's reads and the second
 // launch: where the longest request is two steps of each wave, or four where there are
 // tasks enough for a quarter of the CUs; but not where there are more tasks than two for
-// each CU (of rows of 256 bytes; more of shorter ones), as most waves of a short one have
-// nothing to do. One request of 200 tokens (8 kv heads of 128, bf16) 6.7 us, shared out
-// 9.0; of 1000 14.1 and 9.5; 64 of up to 500 16.3 and 25; 128 of up to 500 39 and 35 (fp8
-// 21 and 27), 256 of up to 60 36 and 25 (fp8 22 and 23).
+// each CU (eight, of rows of 128 bytes and less), as most waves of a short one have
+// nothing to do. 8 kv heads of 128: one request of 200 tokens (bf16) 6.7 us, shared out
+// 9.6; of 1000 13.1 and 9.8; 64 of up to 500 18 and 24; 128 of up to 500 39 and 35 (fp8
+// 22 and 30); 256 of up to 60 36 and 27 (fp8 22 and 28).
 inline bool short_call(long long most, long long tasks, int D, int nt, bool fp8) {
-  if (tasks * (fp8 ? D : 2 * D) > 2 * kCus * 256) return false;
+  if (tasks > ((fp8 ? D : 2 * D) >= 256 ? 2 : 8) * kCus) return false;
   return most <= (tasks >= kCus / 4 ? 4 : 2) * 32 * whole_waves(D, nt);
 }
 
@@ -904,8 +906,10 @@ inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int wi
   if (all * ((rows + 15) / 16) > INT_MAX) return false;
   // Few steps for many rows: 16 rows a task, each reading K and V for itself, rather than
   // more runs for a task and the records of all its rows (28 requests of 702 tokens, 96
-  // rows: 13 us, 22.5 in tasks of 128 rows; 8 of 2000, 48 rows: 14.8 and 13.9).
-  const bool few = all * ((rows + 15) / 16) * steps <= 6LL * per_cu(D, 1) * kCus;
+  // rows of 128 dims: 12 us, 22.8 in tasks of 128 rows; 8 of 2000, 48 rows: 14.9 and 13.9).
+  // Rows of 256 dims leave records twice as large (2 of 8917, 64 rows: 18.4 us, 28.1 in
+  // one task; two tasks read as much more as that saves: 8 of 4000, 32 rows: 26.6, 24.2).
+  const bool few = all * ((rows + 15) / 16) * steps <= (D < 256 ? 18LL : rows > 32 ? 24LL : 6LL) * kCus;
   p->nt = rows <= 16 || D == 256 || few ? 1 : 2;
   const long long sets = (rows + 16 * p->nt - 1) / (16 * p->nt), slots = per_cu(D, p->nt) * kCus;
   p->sets = sets == 1 || few ? 1 : sets == 2 ? 2 : 4;
@@ -913,12 +917,12 @@ inline bool plan_call(int B, int q_len, int Hq, int Hkv, int D, int page, int wi
   const long long blocks = (sets + p->sets - 1) / p->sets;
   p->split = p->sets > 1 || !short_call(most, all * blocks, D, p->nt, fp8);
   // Rows of neighbouring heads: waves that read them together read whole lines and
-  // neighbouring ones (64 requests of 1K..8K tokens, fp8, 8 heads of 128: 122 us, 136
-  // apart). Their records are as many times larger: only where a run then has steps
-  // enough (one request of 20000, windows of 4: 43 us, 32 apart).
+  // neighbouring ones (64 requests of 1K..8K tokens, fp8, 8 heads of 64: 76 us, 100
+  // apart; of 128 112 and 117). Their records are as many times larger: only where a run
+  // then has steps enough (one request of 20000, windows of 4: 28 us, 23 apart).
   if (p->split && by_token)
     while (p->rw < 4 && p->nt == 1 && blocks == 1 && Hkv % (p->rw / p->sets * 2) == 0 &&
-           all / (p->rw / p->sets * 2) * steps >= 16 * slots)
+           all / (p->rw / p->sets * 2) * steps >= 24 * slots)
       p->rw *= 2;
   p->cached = p->sets > 1;
   p->row_blocks = (int)blocks;

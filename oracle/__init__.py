@@ -19,6 +19,8 @@ mla        absorbed-MLA paged decode (reference csrc/mla_decode_a16w8.hip:1-24,
 lite       LiteAttention skip lists: read-row cursor, vote, write-row emitter,
            LPT order (reference csrc/attention_kernel.hip:629-716, :983-995,
            :1296-1347)
+gqa        paged K/V cache of grouped heads, its decode in 64 bits with a bound that
+           counts the kernel's roundings, rotary positions (no reference counterpart)
 
 Pinning: every function is checked in ``tests/test_oracle_*.py`` against
 hand-derived known answers, closed forms or library routines (torch's RTNE

@@ -390,8 +390,8 @@ def test_every_step_is_taken_once(seed):
     for p in parts:
         load[p[0]] = load.get(p[0], 0) + p[4] - p[3]
     order = [p[0] for p in parts]
-    assert order == sorted(order) and order[0] >= 0 and order[-1] < 768
-    mean = sum(-(-n // 32) + 12 for n in lens if n) * per / min(768, max(order) + 1)
+    assert order == sorted(order) and order[0] >= 0 and order[-1] < 512
+    mean = sum(-(-n // 32) + 12 for n in lens if n) * per / min(512, max(order) + 1)
     assert max(load.values()) <= 2 * mean + 20
 
 
