@@ -126,7 +126,8 @@ def gqa_kv_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None) -> N
     A bf16 cache takes the rows as they are. For an fp8 cache each row (token,
     head) gets scale = max(amax / 448, 2^-126), amax over its finite values, and
     codes e4m3fn(x / scale), rounded to nearest even; a value that is not finite
-    becomes NaN. k and v must lie apart from the caches.
+    becomes NaN. k and v must lie apart from the caches, and the K and V caches
+    (and their scales) must not share memory: slices of one tensor are fine.
     """
     if _lib.calls.gqa_write(k, v, k_cache, v_cache, slots, k_scale, v_scale):
         return
@@ -152,7 +153,7 @@ def gqa_kv_read(k_cache, v_cache, slots, k_scale=None, v_scale=None, *, k=None, 
     come twice). An fp8 row is bf16(code * scale), rounded to nearest even. A
     negative slot, or one past the cache, gives a row of zeros. ``k`` and ``v``
     are optional outputs (any strides with a contiguous last dim and rows on
-    16-byte boundaries), apart from the caches.
+    16-byte boundaries), apart from the caches and sharing no memory.
     """
     res = _lib.calls.gqa_read(k_cache, v_cache, slots, k_scale, v_scale, k, v)
     if res is not None:

@@ -302,8 +302,9 @@ int launch_gqa_kv_read(const void* k_cache, const void* v_cache, const void* k_s
  * page]); query head h reads kv head h / (Hq / Hkv). q, out: bf16 [B, q_len, Hq,
  * head_dim] (out may be q); lse: fp32 [B, q_len, Hq] contiguous or NULL, ln of the
  * softmax's sum. A query that sees no token: zeros, -inf. workspace:
- * moonmath_gqa_decode_workspace bytes for the same arguments (NULL where that is 0), 16-byte aligned, its
- * contents neither read nor kept across calls; calls that overlap need one each.
+ * moonmath_gqa_decode_workspace bytes for the same arguments (NULL where that is 0),
+ * 16-byte aligned, its contents neither read nor kept across calls; calls that
+ * overlap need one each.
  * strides: q {batch, query, head}, out {batch, query, head}, k cache, v cache,
  * {block_table row}: 17. */
 int launch_gqa_decode_paged(const void* q, const void* k_cache, const void* v_cache, const void* k_scale,
