@@ -350,6 +350,49 @@ def test_graph_replays():
             assert torch.equal(o[0], want[0]) and torch.equal(o[1], want[1])
 
 
+def test_graphs_of_one_pool():
+    """Graphs that take workspaces and outputs from one pool, replayed one behind the
+    other: each finds what it needs, and the first one's output is read before the next."""
+    states = [_serving(8), _serving(9, B=40, T=1)]
+    want = [_call(s) for s in states]
+    pool = torch.cuda.graph_pool_handle()
+    graphs, outs = [], []
+    for s in states:
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, pool=pool):
+            outs.append(_call(s))
+        graphs.append(g)
+    for i in (0, 1, 1, 0, 0, 1):
+        graphs[i].replay()
+        o, l = (t.clone() for t in outs[i])
+        assert torch.equal(o, want[i][0]) and torch.equal(l, want[i][1])
+
+
+def test_calls_from_two_threads():
+    import threading
+
+    states = [_serving(10), _serving(11, B=40, T=1)]
+    want = [_call(s) for s in states]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = _call(states[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(x, y) for x, y in zip(got, want[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_parts_join_by_their_sums():
     """A context cut at a page: its parts' outputs joined by their lse equal the whole's."""
     k, v, _, _ = cache(32, 2, 64, 128, False, 11)
